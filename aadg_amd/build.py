@@ -16,7 +16,10 @@ INCLUDE = os.path.join(os.path.dirname(_HERE), "include")
 
 # -ffp-contract=off: the uint8 path restates Pillow's double/float expressions operation by
 # operation; FMA contraction would change roundings.  Kernels that want FMAs call fmaf explicitly.
+# -packed-fp32-ops: some forms of the packed float32 instructions that -O3 makes from ordinary float code are not reliable on this part
+# (hipcc's host pass warns that it does not know the feature: harmless).
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                "-Wall", "-Wno-unused-function", "-I" + INCLUDE, "-I" + CSRC]
 
 
