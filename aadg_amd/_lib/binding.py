@@ -60,6 +60,8 @@ EXPORTS = [
     "aadg_bn_finalize_f32", "aadg_conv1x1_f32x3_pre_supported", "aadg_conv1x1_nchw_f32x3_pre", "aadg_conv1x1_wgrad_f32x3_pre",
     "aadg_conv3x3_nchw_f32x3_pre", "aadg_conv3x3_wgrad_f32x3_pre", "aadg_conv1x1_wgrad_f32x3_pre_supported", "aadg_bn_forward_res_affine_f32", "aadg_bn_backward_res_bn_f32",
     "aadg_bn_sync_backward_res_bn_f32", "aadg_draw_python_stream",
+    "aadg_attention_supported", "aadg_attention_forward_workspace_bytes", "aadg_attention_forward",
+    "aadg_attention_backward_workspace_bytes", "aadg_attention_backward",
 ]
 
 _lib = None
@@ -292,6 +294,16 @@ def load():
     lib.aadg_conv3x3s2_dgrad_f32x3.argtypes = [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]
     lib.aadg_conv3x3s2_wgrad_f32x3.restype = _i
     lib.aadg_conv3x3s2_wgrad_f32x3.argtypes = [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]
+    lib.aadg_attention_supported.restype = _i
+    lib.aadg_attention_supported.argtypes = [_vp]
+    lib.aadg_attention_forward_workspace_bytes.restype = _sz
+    lib.aadg_attention_forward_workspace_bytes.argtypes = [_vp]
+    lib.aadg_attention_forward.restype = _i
+    lib.aadg_attention_forward.argtypes = [_vp] * 8 + [_sz, _vp]
+    lib.aadg_attention_backward_workspace_bytes.restype = _sz
+    lib.aadg_attention_backward_workspace_bytes.argtypes = [_vp]
+    lib.aadg_attention_backward.restype = _i
+    lib.aadg_attention_backward.argtypes = [_vp] * 12 + [_sz, _vp]
     if lib.aadg_abi_version() != 12:
         raise RuntimeError("libaadg_hip.so ABI version mismatch")
     _lib = lib

@@ -1,0 +1,761 @@
+// Softmax attention, forward and backward, for the transformer blocks of the SegFormer backbone (reference:
+// models/mmseg/models/backbones/mix_transformer.py:86-100 `attn = (q @ k^T) * scale; softmax; attn @ v`).
+//
+//   s_ij = scale q_i . k_j            allowed(i, j): j < L_b  and  (not causal or j <= i + L_b - Nq)
+//   lse_i = log sum_allowed exp s_ij  p_ij = exp(s_ij - lse_i)      o_i = sum_j p_ij v_j        (no allowed key: o_i = 0)
+//   D_i = do_i . o_i                  ds_ij = p_ij (do_i . v_j - D_i)
+//   dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i      dv_j = sum_i p_ij do_i
+//
+// The score matrix never reaches memory: the forward keeps a running maximum and sum per row (one pass over the keys) and leaves
+// lse_i in base 2 (4 bytes a row), from which the backward recomputes p.
+//
+// Heads that share one key head (H = G r) are FOLDED into the rows: a workgroup of group g works on the R = r Nq rows
+// (head g r + row / Nq, query row % Nq), so the keys are read once for all of them and the sums of dk / dv over the shared heads
+// are part of the same accumulation.
+//
+// Matrix-core layout (one code for both types, template parameter T).  C of a 32 x 32 product: lane & 31 = column, register r of lane
+// half h = row 8 (r / 4) + 4 h + r % 4.  The scores are taken TRANSPOSED where a lane must own a query (forward, dq: columns =
+// queries, the row maximum and sum are in-register plus one exchange of the halves) and straight where a lane must own a key (dk,
+// dv).  Either way the probabilities are the next product's B operand as they lie in the registers: the k slots of an MFMA are
+// summed over, so any order of them is right as long as A uses the same one -- a B fragment made of C registers has slot (h, e) =
+// row 4 h + e (and 8 + 4 h + e), and the A fragment is read from LDS for those rows.
+//   bfloat16: v_mfma_f32_32x32x16_bf16, fragments of 8 values; the transposed A operand with ds_read_b64_tr_b16.
+//   float32:  v_mfma_f32_32x32x2_f32, four per fragment of 4 values: exact float32 products (scores go through an exponential: a product
+//             split in two bfloat16 halves, 2^-17 relative, would move p by |s| 2^-17).
+// The probabilities and ds are rounded to bfloat16 for the second products of the bfloat16 kernels (half a step, 2^-8 relative, of
+// factors whose partner is bfloat16 as well); maxima, sums, lse, D and every accumulator are float32.
+#include "common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 at_bf16x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef uint32_t at_u32x4 __attribute__((ext_vector_type(4)));
+typedef short at_v4i16 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }     // v_exp_f32: 1 ulp, results below 2^-126 are 0
+
+constexpr float AT_LOG2E = 1.4426950408889634f;
+
+struct AtStride { long long b, h, n; };               // elements: batch, head, row (the head dimension itself is contiguous)
+
+struct AtArgs {
+    const void *q, *k, *v, *o, *dout;
+    void *out, *dq, *dk, *dv;                         // out: o (forward)
+    const int* key_lengths;
+    float* lse;                                       // [B, H, Nq] base-2 log-sum-exp; +inf for a row without keys
+    float* delta;                                     // [B, H, Nq] D_i (backward)
+    float *part, *ml;                                 // split partials: [splits][rows][d] and [splits][rows][2]
+    AtStride sq, sk, sv, so, sdo, sdq, sdk, sdv;
+    int B, H, G, Nq, Nk, d, causal, r, R;
+    int tiles, splits, chunk;                         // row (or key) tiles per group, splits of the loop axis, its length per split
+    float scale;
+};
+
+template <typename T> struct At;
+template <> struct At<uint16_t> {
+    static constexpr int KS = 16, CH = 8;             // values of the contracted axis per fragment; elements per 16 bytes
+    typedef at_bf16x8 Frag;
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Frag pack(const f32x16& c, int g) {
+        const at_u32x4 p = {aadg_f2bf_pk(c[8 * g], c[8 * g + 1]), aadg_f2bf_pk(c[8 * g + 2], c[8 * g + 3]),
+                            aadg_f2bf_pk(c[8 * g + 4], c[8 * g + 5]), aadg_f2bf_pk(c[8 * g + 6], c[8 * g + 7])};
+        return __builtin_bit_cast(Frag, p);
+    }
+    static __device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(aadg_f2bf_pk(a, b), aadg_f2bf_pk(c, d));
+    }
+};
+template <> struct At<float> {
+    static constexpr int KS = 8, CH = 4;
+    typedef aadg_f32x4 Frag;
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ Frag pack(const f32x16& c, int g) { return Frag{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]}; }
+    static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+        *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+    }
+};
+
+// A tile of rows x D in LDS, row-major.  bfloat16: no padding, the 16-byte chunks of a row permuted by a function of the row such that
+// both the row reads (8 rows, one chunk) and the transpose reads (4 rows, 4 neighbouring chunks) touch every bank once.
+// float32: pitch D + 8 words (row reads of 16 bytes: 8 banks apart; column reads: the two halves, 4 rows apart, 32 banks apart).
+template <typename T, int D> struct Tile;
+template <int D> struct Tile<uint16_t, D> {
+    static constexpr int PITCH = D;
+    static __device__ __forceinline__ int swz(int row) {
+        return D == 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : D == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : ((row >> 2) & 3);
+    }
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * D + ((chunk ^ swz(row)) << 3); }
+    // rows row0 + (lane & 31), values KS u + 8 h .. + 7
+    static __device__ __forceinline__ at_bf16x8 rows(const uint16_t* t, int row0, int u, int lane) {
+        return __builtin_bit_cast(at_bf16x8, *reinterpret_cast<const at_u32x4*>(t + at(row0 + (lane & 31), 2 * u + (lane >> 5))));
+    }
+    // column c0 + (lane & 31), rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3}: ds_read_b64_tr_b16 gives lane i of 16 the 4 rows of
+    // column i; the lane passes the address of row i / 4, columns 4 (i % 4)
+    static __device__ __forceinline__ at_bf16x8 cols(const uint16_t* t, int row0, int c0, int lane) {
+        const int i = lane & 15, row = row0 + 4 * (lane >> 5) + (i >> 2), c = c0 + (lane & 16) + 4 * (i & 3);
+        const uint16_t* p0 = t + at(row, c >> 3) + (c & 7);
+        const uint16_t* p1 = t + at(row + 8, c >> 3) + (c & 7);
+        typedef at_v4i16 __attribute__((address_space(3)))* lds_p;
+        const at_v4i16 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p0)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p1));
+        typedef short v8i16 __attribute__((ext_vector_type(8)));
+        const v8i16 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        return __builtin_bit_cast(at_bf16x8, v);
+    }
+};
+template <int D> struct Tile<float, D> {
+    static constexpr int PITCH = D + 8;
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * PITCH + (chunk << 2); }
+    static __device__ __forceinline__ aadg_f32x4 rows(const float* t, int row0, int u, int lane) {
+        return *reinterpret_cast<const aadg_f32x4*>(t + at(row0 + (lane & 31), 2 * u + (lane >> 5)));
+    }
+    static __device__ __forceinline__ aadg_f32x4 cols(const float* t, int row0, int c0, int lane) {
+        const float* p = t + (row0 + 4 * (lane >> 5)) * PITCH + c0 + (lane & 31);
+        return aadg_f32x4{p[0], p[PITCH], p[2 * PITCH], p[3 * PITCH]};
+    }
+};
+
+// 16 bytes of row `row`, chunk c, of a strided matrix; zero outside rows < n, values < d (the address is clamped, never out of range)
+template <typename T>
+__device__ __forceinline__ uint4 at_load(const T* base, long long stride, int row, int n, int c, int d) {
+    const int col = c * At<T>::CH;
+    const bool ok = row < n && col < d;
+    const uint4 x = *reinterpret_cast<const uint4*>(base + (long long)(row < n ? row : n - 1) * stride + (col < d ? col : 0));
+    return ok ? x : make_uint4(0, 0, 0, 0);
+}
+
+// folded row -> element offset of a [B, H, Nq] strided matrix for group g
+__device__ __forceinline__ long long at_row(const AtArgs& a, const AtStride& s, int b, int g, int row) {
+    const int hr = a.r == 1 ? 0 : row / a.Nq, i = row - hr * a.Nq;
+    return b * s.b + (long long)(g * a.r + hr) * s.h + (long long)i * s.n;
+}
+__device__ __forceinline__ int at_query(const AtArgs& a, int row) { return a.r == 1 ? row : row % a.Nq; }
+
+__device__ __forceinline__ int at_len(const AtArgs& a, int b) {
+    return a.key_lengths == nullptr ? a.Nk : max(0, min(a.Nk, a.key_lengths[b]));
+}
+
+// keys a folded row sees: [0, at_limit)
+__device__ __forceinline__ int at_limit(const AtArgs& a, int L, int row) {
+    return a.causal ? max(0, min(L, at_query(a, row) + L - a.Nq + 1)) : L;
+}
+
+// the largest limit of rows [row0, row0 + n): the last one's, or L if the range holds the last query of a head
+__device__ __forceinline__ int at_limit_max(const AtArgs& a, int L, int row0, int n) {
+    const int last = min(row0 + n, a.R) - 1;
+    if (!a.causal) return L;
+    if (a.r > 1 && row0 / a.Nq != last / a.Nq) return L;
+    return at_limit(a, L, last);
+}
+
+// keys per LDS tile: 64; 32 where the next tile's prefetch registers (2 BK D / threads values) would not fit beside the accumulators
+template <typename T, int D, int NW> constexpr int at_bk() { return NW == 1 || (sizeof(T) == 4 && D == 128) ? 32 : 64; }
+
+// ------------------------------------------------------------------------------------------------ forward
+// Workgroup: NW waves of 32 folded rows; keys in tiles of BK through LDS, the next tile's loads in registers during the products.
+template <typename T, int D, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AtArgs a) {
+    typedef At<T> M;
+    typedef Tile<T, D> L_;
+    constexpr int BK = at_bk<T, D, NW>(), KS = M::KS, CH = M::CH, U = D / KS, CPR = D / CH, NT = 64 * NW, LD = BK * CPR / NT, DT = D / 32, PG = 16 / (KS / 2), KT = BK / 32;
+    __shared__ __attribute__((aligned(16))) T Ks[BK * L_::PITCH];
+    __shared__ __attribute__((aligned(16))) T Vs[BK * L_::PITCH];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    const int sp = SPLIT ? blockIdx.x % a.splits : 0;
+    const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
+    const int bg = w / a.tiles, tile = a.tiles - 1 - (w - bg * a.tiles), b = bg / a.G, g = bg - b * a.G;      // causal: longest rows first
+    const int L = at_len(a, b);
+    const int row0 = tile * 32 * NW + 32 * wv, row = row0 + (lane & 31);
+    const bool live = row < a.R;
+    const int k_lo = SPLIT ? sp * a.chunk : 0;
+    const int wg_end = min(at_limit_max(a, L, tile * 32 * NW, 32 * NW), SPLIT ? k_lo + a.chunk : L);
+    const int limit = live ? at_limit(a, L, row) : 0;
+    const int wave_end = row0 < a.R ? at_limit_max(a, L, row0, 32) : 0;
+    int wave_full = limit;                                                    // keys every row of the wave sees
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) wave_full = min(wave_full, __shfl_xor(wave_full, o, 64));
+
+    const T* kb = (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
+    const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
+    typename M::Frag qf[U];
+    {
+        const T* qp = (const T*)a.q + at_row(a, a.sq, b, g, live ? row : 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) qf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(qp, 0, live ? 0 : 1, 1, 2 * u + h, a.d));
+    }
+    f32x16 acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const float c = a.scale * AT_LOG2E;
+
+    uint4 rk[LD], rv[LD];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
+            rk[i] = at_load<T>(kb, a.sk.n, k0 + rw, L, ch, a.d);
+            rv[i] = at_load<T>(vb, a.sv.n, k0 + rw, L, ch, a.d);
+        }
+    };
+    if (k_lo < wg_end) fetch(k_lo);
+    for (int k0 = k_lo; k0 < wg_end; k0 += BK) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
+            *reinterpret_cast<uint4*>(&Ks[L_::at(rw, ch)]) = rk[i];
+            *reinterpret_cast<uint4*>(&Vs[L_::at(rw, ch)]) = rv[i];
+        }
+        __syncthreads();
+        if (k0 + BK < wg_end) fetch(k0 + BK);
+        if (k0 >= wave_end) continue;                                         // (wave-uniform; the barriers above are reached by all)
+        f32x16 s[KT];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[t] = M::mma(L_::rows(Ks, 32 * t, u, lane), qf[u], s[t]);
+        }
+        if (k0 + BK > wave_full) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[t][i] = k0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) < limit ? s[t][i] : -INFINITY;
+        }
+        float mx = m;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mc = mx == -INFINITY ? 0.0f : mx * c;
+        const float alpha = at_exp2(fmaf(m, c, -mc));
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[t][i] = at_exp2(fmaf(s[t][i], c, -mc));
+                sum += s[t][i];
+            }
+        l = fmaf(l, alpha, sum);
+        m = mx;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int p = 0; p < PG; ++p) {
+                const typename M::Frag pf = M::pack(s[t], p);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) acc[dt] = M::mma(L_::cols(Vs, 32 * t + KS * p, 32 * dt, lane), pf, acc[dt]);
+            }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (!live) return;
+    const long long flat = ((long long)b * a.G + g) * a.R + row;              // = (b H + head) Nq + query
+    if (SPLIT) {
+        const long long rows = (long long)a.B * a.G * a.R;
+        if (h == 0) {
+            a.ml[2 * (sp * rows + flat)] = m * c;
+            a.ml[2 * (sp * rows + flat) + 1] = l;
+        }
+        float* op = a.part + (sp * rows + flat) * a.d;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int col = 32 * t + 8 * i + 4 * h;
+                if (col < a.d) *reinterpret_cast<float4*>(op + col) = make_float4(acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]);
+            }
+        return;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);           // NaN stays
+    T* op = (T*)a.out + at_row(a, a.so, b, g, row);
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = 32 * t + 8 * i + 4 * h;
+            if (col < a.d) M::store4(op + col, acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv, acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv);
+        }
+    if (h == 0 && a.lse != nullptr) a.lse[flat] = l == 0.0f ? INFINITY : fmaf(m, c, log2f(l));
+}
+
+// joins the splits of the forward: one lane per 4 values of a row
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_join(const AtArgs a) {
+    const int per = a.d / 4;
+    const long long rows = (long long)a.B * a.G * a.R, id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long flat = id / per;
+    if (flat >= rows) return;
+    const int col = (int)(id - flat * per) * 4;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s)
+        if (a.ml[2 * (s * rows + flat) + 1] != 0.0f) m = fmaxf(m, a.ml[2 * (s * rows + flat)]);
+    float l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int s = 0; s < a.splits; ++s) {
+        const float ls = a.ml[2 * (s * rows + flat) + 1];
+        if (ls == 0.0f) continue;                                             // no key of this split
+        const float w = at_exp2(a.ml[2 * (s * rows + flat)] - m);
+        const float4 x = *reinterpret_cast<const float4*>(a.part + (s * rows + flat) * a.d + col);
+        l = fmaf(ls, w, l);
+        o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+    }
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    const long long bg = flat / a.R;
+    const int b = (int)(bg / a.G), g = (int)(bg - (long long)b * a.G), row = (int)(flat - bg * a.R);
+    At<T>::store4((T*)a.out + at_row(a, a.so, b, g, row) + col, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (col == 0 && a.lse != nullptr) a.lse[flat] = l == 0.0f ? INFINITY : m + log2f(l);
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// D_i = do_i . o_i, one 16-lane group per row
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
+    const long long rows = (long long)a.B * a.G * a.R, flat = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (flat >= rows) return;
+    const long long bg = flat / a.R;
+    const int b = (int)(bg / a.G), g = (int)(bg - (long long)b * a.G), row = (int)(flat - bg * a.R);
+    const T* op = (const T*)a.o + at_row(a, a.so, b, g, row);
+    const T* gp = (const T*)a.dout + at_row(a, a.sdo, b, g, row);
+    float s = 0.0f;
+    for (int c = threadIdx.x & 15; c * At<T>::CH < a.d; c += 16) {
+        const uint4 x = *reinterpret_cast<const uint4*>(op + c * At<T>::CH), y = *reinterpret_cast<const uint4*>(gp + c * At<T>::CH);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (At<T>::CH == 4) {
+                s = fmaf(__uint_as_float(xs[i]), __uint_as_float(ys[i]), s);
+            } else {
+                s = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), s);
+                s = fmaf(__uint_as_float(xs[i] & 0xFFFF0000u), __uint_as_float(ys[i] & 0xFFFF0000u), s);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 15) == 0) a.delta[flat] = s;
+}
+
+// dq: the forward's walk over the keys with p recomputed; dq^T += K^T ds^T
+template <typename T, int D, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void k_attn_dq(const AtArgs a) {
+    typedef At<T> M;
+    typedef Tile<T, D> L_;
+    constexpr int BK = at_bk<T, D, NW>(), KS = M::KS, CH = M::CH, U = D / KS, CPR = D / CH, NT = 64 * NW, LD = BK * CPR / NT, DT = D / 32, PG = 16 / (KS / 2), KT = BK / 32;
+    __shared__ __attribute__((aligned(16))) T Ks[BK * L_::PITCH];
+    __shared__ __attribute__((aligned(16))) T Vs[BK * L_::PITCH];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    const int sp = SPLIT ? blockIdx.x % a.splits : 0;
+    const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
+    const int bg = w / a.tiles, tile = a.tiles - 1 - (w - bg * a.tiles), b = bg / a.G, g = bg - b * a.G;
+    const int L = at_len(a, b);
+    const int row0 = tile * 32 * NW + 32 * wv, row = row0 + (lane & 31);
+    const bool live = row < a.R;
+    const int k_lo = SPLIT ? sp * a.chunk : 0;
+    const int wg_end = min(at_limit_max(a, L, tile * 32 * NW, 32 * NW), SPLIT ? k_lo + a.chunk : L);
+    const int limit = live ? at_limit(a, L, row) : 0;
+    const int wave_end = row0 < a.R ? at_limit_max(a, L, row0, 32) : 0;
+    int wave_full = limit;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) wave_full = min(wave_full, __shfl_xor(wave_full, o, 64));
+    const T* kb = (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
+    const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
+    const long long flat = ((long long)b * a.G + g) * a.R + row;
+    typename M::Frag qf[U], gf[U];
+    {
+        const T* qp = (const T*)a.q + at_row(a, a.sq, b, g, live ? row : 0);
+        const T* gp = (const T*)a.dout + at_row(a, a.sdo, b, g, live ? row : 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            qf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(qp, 0, live ? 0 : 1, 1, 2 * u + h, a.d));
+            gf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(gp, 0, live ? 0 : 1, 1, 2 * u + h, a.d));
+        }
+    }
+    const float lse = live ? a.lse[flat] : INFINITY, dl = live ? a.delta[flat] : 0.0f;
+    const float c = a.scale * AT_LOG2E;
+    f32x16 acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    uint4 rk[LD], rv[LD];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
+            rk[i] = at_load<T>(kb, a.sk.n, k0 + rw, L, ch, a.d);
+            rv[i] = at_load<T>(vb, a.sv.n, k0 + rw, L, ch, a.d);
+        }
+    };
+    if (k_lo < wg_end) fetch(k_lo);
+    for (int k0 = k_lo; k0 < wg_end; k0 += BK) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
+            *reinterpret_cast<uint4*>(&Ks[L_::at(rw, ch)]) = rk[i];
+            *reinterpret_cast<uint4*>(&Vs[L_::at(rw, ch)]) = rv[i];
+        }
+        __syncthreads();
+        if (k0 + BK < wg_end) fetch(k0 + BK);
+        if (k0 >= wave_end) continue;
+        const bool edge = k0 + BK > wave_full;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s = M::mma(L_::rows(Ks, 32 * t, u, lane), qf[u], s);
+                dp = M::mma(L_::rows(Vs, 32 * t, u, lane), gf[u], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = at_exp2(fmaf(s[i], c, -lse)) * (dp[i] - dl);
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = k0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) < limit ? s[i] : 0.0f;
+            }
+#pragma unroll
+            for (int p = 0; p < PG; ++p) {
+                const typename M::Frag pf = M::pack(s, p);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) acc[dt] = M::mma(L_::cols(Ks, 32 * t + KS * p, 32 * dt, lane), pf, acc[dt]);
+            }
+        }
+    }
+    if (!live) return;
+    const float sc = a.scale;
+    T* op = (T*)a.dq + at_row(a, a.sdq, b, g, row);
+    float* pp = SPLIT ? a.part + (sp * ((long long)a.B * a.G * a.R) + flat) * a.d : nullptr;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = 32 * t + 8 * i + 4 * h;
+            if (col >= a.d) continue;
+            const float x = acc[t][4 * i] * sc, y = acc[t][4 * i + 1] * sc, z = acc[t][4 * i + 2] * sc, q = acc[t][4 * i + 3] * sc;
+            if (SPLIT) *reinterpret_cast<float4*>(pp + col) = make_float4(x, y, z, q);
+            else M::store4(op + col, x, y, z, q);
+        }
+}
+
+// dk, dv: a wave owns 32 keys (its K and V fragments stay in registers) and walks the folded rows in tiles of 32;
+// dv^T += dO^T P, dk^T += Q^T dS
+template <typename T, int D, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AtArgs a) {
+    typedef At<T> M;
+    typedef Tile<T, D> L_;
+    constexpr int BQ = 32, KS = M::KS, CH = M::CH, U = D / KS, CPR = D / CH, NT = 64 * NW, LD = (BQ * CPR + NT - 1) / NT, DT = D / 32, PG = 16 / (KS / 2);
+    __shared__ __attribute__((aligned(16))) T Qs[BQ * L_::PITCH];
+    __shared__ __attribute__((aligned(16))) T Gs[BQ * L_::PITCH];
+    __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
+    __shared__ int Es[BQ];                                                   // key limit of each row
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    const int sp = SPLIT ? blockIdx.x % a.splits : 0;
+    const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
+    const int bg = w / a.tiles, tile = w - bg * a.tiles, b = bg / a.G, g = bg - b * a.G;
+    const int L = at_len(a, b);
+    const int key0 = tile * 32 * NW + 32 * wv, key = key0 + (lane & 31);
+    const T* kb = (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
+    const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
+    const float c = a.scale * AT_LOG2E;
+    const int r_lo = SPLIT ? sp * a.chunk : 0, r_hi = SPLIT ? min(a.R, r_lo + a.chunk) : a.R;
+    const bool any = tile * 32 * NW < L;                                      // (workgroup-uniform)
+    typename M::Frag kf[U], vf[U];
+    if (any) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            kf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(kb, a.sk.n, key, L, 2 * u + h, a.d));
+            vf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(vb, a.sv.n, key, L, 2 * u + h, a.d));
+        }
+    }
+    f32x16 ak[DT], av[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ak[t][i] = av[t][i] = 0.0f;
+    if (any) {
+        for (int q0 = r_lo; q0 < r_hi; q0 += BQ) {
+            if (a.causal && at_limit_max(a, L, q0, BQ) <= tile * 32 * NW) continue;      // (workgroup-uniform) no row of the tile sees a key of this workgroup
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < LD; ++i) {
+                const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
+                if (id >= BQ * CPR) break;
+                const int rr = q0 + rw;
+                const bool ok = rr < r_hi;
+                const uint4 x = at_load<T>((const T*)a.q + at_row(a, a.sq, b, g, ok ? rr : q0), 0, ok ? 0 : 1, 1, ch, a.d);
+                const uint4 y = at_load<T>((const T*)a.dout + at_row(a, a.sdo, b, g, ok ? rr : q0), 0, ok ? 0 : 1, 1, ch, a.d);
+                *reinterpret_cast<uint4*>(&Qs[L_::at(rw, ch)]) = x;
+                *reinterpret_cast<uint4*>(&Gs[L_::at(rw, ch)]) = y;
+            }
+            if (tid < BQ) {
+                const int rr = q0 + tid;
+                const bool ok = rr < r_hi;
+                const long long f = ((long long)b * a.G + g) * a.R + (ok ? rr : q0);
+                Ls[tid] = ok ? a.lse[f] : INFINITY;
+                Ds[tid] = ok ? a.delta[f] : 0.0f;
+                Es[tid] = ok ? at_limit(a, L, rr) : 0;
+            }
+            __syncthreads();
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s = M::mma(L_::rows(Qs, 0, u, lane), kf[u], s);
+                dp = M::mma(L_::rows(Gs, 0, u, lane), vf[u], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int rr = 8 * (i >> 2) + 4 * h + (i & 3);
+                const float p = key < Es[rr] ? at_exp2(fmaf(s[i], c, -Ls[rr])) : 0.0f;
+                s[i] = p;
+                dp[i] = key < Es[rr] ? p * (dp[i] - Ds[rr]) : 0.0f;
+            }
+#pragma unroll
+            for (int p = 0; p < PG; ++p) {
+                const typename M::Frag pf = M::pack(s, p), df = M::pack(dp, p);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    av[dt] = M::mma(L_::cols(Gs, KS * p, 32 * dt, lane), pf, av[dt]);
+                    ak[dt] = M::mma(L_::cols(Qs, KS * p, 32 * dt, lane), df, ak[dt]);
+                }
+            }
+        }
+    }
+    if (key >= a.Nk) return;
+    const float sc = a.scale;
+    const long long rows = (long long)a.B * a.G * a.Nk, flat = ((long long)b * a.G + g) * a.Nk + key;
+    T* kp = (T*)a.dk + b * a.sdk.b + (long long)g * a.sdk.h + (long long)key * a.sdk.n;
+    T* vp = (T*)a.dv + b * a.sdv.b + (long long)g * a.sdv.h + (long long)key * a.sdv.n;
+    float* pk = SPLIT ? a.part + (2 * sp * rows + flat) * a.d : nullptr;
+    float* pv = SPLIT ? pk + rows * a.d : nullptr;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = 32 * t + 8 * i + 4 * h;
+            if (col >= a.d) continue;
+            const float4 x = make_float4(ak[t][4 * i] * sc, ak[t][4 * i + 1] * sc, ak[t][4 * i + 2] * sc, ak[t][4 * i + 3] * sc);
+            const float4 y = make_float4(av[t][4 * i], av[t][4 * i + 1], av[t][4 * i + 2], av[t][4 * i + 3]);
+            if (SPLIT) {
+                *reinterpret_cast<float4*>(pk + col) = x;
+                *reinterpret_cast<float4*>(pv + col) = y;
+            } else {
+                M::store4(kp + col, x.x, x.y, x.z, x.w);
+                M::store4(vp + col, y.x, y.y, y.z, y.w);
+            }
+        }
+}
+
+// sum of the splits' partials in split order, one lane per 4 values: out[b, head, n] = sum_s part[s * step + (b heads + head) n_rows + n]
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_sum(const float* __restrict__ part, T* __restrict__ out, AtStride s, int B, int heads, int n_rows,
+                                                  int d, int splits, long long step) {
+    const int per = d / 4;
+    const long long rows = (long long)B * heads * n_rows, id = (long long)blockIdx.x * 256 + threadIdx.x, flat = id / per;
+    if (flat >= rows) return;
+    const int col = (int)(id - flat * per) * 4;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int i = 0; i < splits; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(part + i * step + flat * d + col);
+        o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+    }
+    const long long bh = flat / n_rows;
+    const long long b = bh / heads, hh = bh - b * heads, n = flat - bh * n_rows;
+    At<T>::store4(out + b * s.b + hh * s.h + n * s.n + col, o.x, o.y, o.z, o.w);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+constexpr int AT_TARGET_WG = 512;                     // two workgroups of 4 waves per CU
+
+AtStride at_stride(const int64_t* s) { return AtStride{s[0], s[1], s[2]}; }
+
+// 0, or the error of a descriptor the kernels do not take.  16-byte rows: every stride and pointer a multiple of 16 bytes.
+int at_check(const aadg_attention_desc* s) {
+    if (s == nullptr || s->dtype < 0 || s->dtype > 1 || s->B < 1 || s->H < 1 || s->G < 1 || s->Nq < 1 || s->Nk < 1 || s->d < 1) return AADG_E_BADARG;
+    if (!(s->scale > 0.0f) || !(s->scale < INFINITY)) return AADG_E_BADARG;
+    if (s->H % s->G != 0) return AADG_E_BADARG;
+    if (s->d % 8 != 0 || s->d > 128) return AADG_E_UNSUPPORTED;
+    const int64_t r = s->H / s->G, R = r * s->Nq;
+    if (R > (1 << 30) || s->Nk > (1 << 30) || (int64_t)s->B * s->H > (1 << 20)) return AADG_E_UNSUPPORTED;
+    // grids: at most (rows or keys) / 32 tiles per group, 64 splits
+    if ((int64_t)s->B * s->G * (((R > s->Nk ? R : s->Nk) + 31) / 32) * 64 > 0x7FFFFFFF) return AADG_E_UNSUPPORTED;
+    if ((int64_t)s->B * s->H * s->Nq * (s->d / 4) / 256 >= 0x7FFFFFFF || (int64_t)s->B * s->G * s->Nk * (s->d / 4) / 256 >= 0x7FFFFFFF) return AADG_E_UNSUPPORTED;
+    return 0;
+}
+bool at_aligned(const aadg_attention_desc* s, const void* p, const int64_t* st) {
+    const int unit = s->dtype == 1 ? 8 : 4;
+    return p != nullptr && (uintptr_t)p % 16 == 0 && st[0] % unit == 0 && st[1] % unit == 0 && st[2] % unit == 0;
+}
+
+struct AtPlan { int nw, tiles, splits, chunk; };
+
+// waves per workgroup by what there is to own (32 rows a wave); splits of the other axis (in units of `tile`) until the card has
+// AT_TARGET_WG workgroups' worth of waves, each with at least two tiles to amortise the join
+AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile) {
+    AtPlan p;
+    p.nw = own <= 32 ? 1 : 4;
+    p.tiles = (own + 32 * p.nw - 1) / (32 * p.nw);
+    const int64_t waves = (int64_t)s->B * s->G * p.tiles * p.nw;
+    const int n = (other + tile - 1) / tile;
+    int64_t sp = (4 * AT_TARGET_WG + waves - 1) / waves;
+    if (sp > n / 2) sp = n / 2;
+    if (sp > 64) sp = 64;
+    if (sp < 1) sp = 1;
+    const int per = (int)((n + sp - 1) / sp);
+    p.chunk = per * tile;
+    p.splits = (n + per - 1) / per;
+    return p;
+}
+AtPlan at_plan_rows(const aadg_attention_desc* s) { return at_plan(s, s->H / s->G * s->Nq, s->Nk, 64); }
+AtPlan at_plan_keys(const aadg_attention_desc* s) { return at_plan(s, s->Nk, s->H / s->G * s->Nq, 32); }
+
+size_t at_fwd_bytes(const aadg_attention_desc* s) {
+    const AtPlan p = at_plan_rows(s);
+    return p.splits > 1 ? (size_t)p.splits * s->B * s->H * s->Nq * (s->d + 2) * 4 : 0;
+}
+
+void at_fill(AtArgs& a, const aadg_attention_desc* s, const int* key_lengths) {
+    a.key_lengths = key_lengths;
+    a.B = s->B; a.H = s->H; a.G = s->G; a.Nq = s->Nq; a.Nk = s->Nk; a.d = s->d; a.causal = s->causal != 0;
+    a.r = s->H / s->G; a.R = a.r * s->Nq; a.scale = s->scale;
+    a.sq = at_stride(s->q_stride); a.sk = at_stride(s->k_stride); a.sv = at_stride(s->v_stride); a.so = at_stride(s->o_stride);
+    a.sdo = at_stride(s->do_stride); a.sdq = at_stride(s->dq_stride); a.sdk = at_stride(s->dk_stride); a.sdv = at_stride(s->dv_stride);
+}
+void at_use(AtArgs& a, const AtPlan& p) { a.tiles = p.tiles; a.splits = p.splits; a.chunk = p.chunk; }
+
+#define AT_LAUNCH(KERNEL, T, D, NW)                                                                                        \
+    do {                                                                                                                   \
+        const dim3 grid((unsigned)((long long)a.B * a.G * p.tiles * p.splits));                                            \
+        if (p.splits > 1) hipLaunchKernelGGL((KERNEL<T, D, NW, true>), grid, dim3(64 * NW), 0, st, a);                     \
+        else hipLaunchKernelGGL((KERNEL<T, D, NW, false>), grid, dim3(64 * NW), 0, st, a);                                 \
+    } while (0)
+#define AT_BY_NW(KERNEL, T, D)                                                                                             \
+    do {                                                                                                                   \
+        if (p.nw == 1) AT_LAUNCH(KERNEL, T, D, 1);                                                                         \
+        else AT_LAUNCH(KERNEL, T, D, 4);                                                                                   \
+    } while (0)
+#define AT_BY_D(KERNEL, T)                                                                                                 \
+    do {                                                                                                                   \
+        if (a.d <= 32) AT_BY_NW(KERNEL, T, 32);                                                                            \
+        else if (a.d <= 64) AT_BY_NW(KERNEL, T, 64);                                                                       \
+        else AT_BY_NW(KERNEL, T, 128);                                                                                     \
+    } while (0)
+
+template <typename T> int at_forward(AtArgs& a, const AtPlan& p, hipStream_t st) {
+    at_use(a, p);
+    AT_BY_D(k_attn_fwd, T);
+    AADG_LAUNCH_CHECK();
+    if (p.splits > 1) {
+        const long long n = (long long)a.B * a.H * a.Nq * (a.d / 4);
+        hipLaunchKernelGGL(k_attn_join<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+        AADG_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, hipStream_t st) {
+    const long long rows = (long long)a.B * a.H * a.Nq;
+    hipLaunchKernelGGL(k_attn_delta<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
+    AADG_LAUNCH_CHECK();
+    if (a.dk != nullptr) {
+        const AtPlan p = at_plan_keys(s);
+        at_use(a, p);
+        AT_BY_D(k_attn_dkv, T);
+        AADG_LAUNCH_CHECK();
+        if (p.splits > 1) {
+            const long long nk = (long long)a.B * a.G * a.Nk, n = nk * (a.d / 4);
+            const dim3 grid((unsigned)((n + 255) / 256));
+            hipLaunchKernelGGL(k_attn_sum<T>, grid, dim3(256), 0, st, a.part, (T*)a.dk, a.sdk, a.B, a.G, a.Nk, a.d, p.splits, 2 * nk * a.d);
+            AADG_LAUNCH_CHECK();
+            hipLaunchKernelGGL(k_attn_sum<T>, grid, dim3(256), 0, st, a.part + nk * a.d, (T*)a.dv, a.sdv, a.B, a.G, a.Nk, a.d, p.splits, 2 * nk * a.d);
+            AADG_LAUNCH_CHECK();
+        }
+    }
+    if (a.dq != nullptr) {
+        const AtPlan p = at_plan_rows(s);
+        at_use(a, p);
+        AT_BY_D(k_attn_dq, T);
+        AADG_LAUNCH_CHECK();
+        if (p.splits > 1) {
+            const long long n = rows * (a.d / 4);
+            hipLaunchKernelGGL(k_attn_sum<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a.part, (T*)a.dq, a.sdq, a.B, a.H, a.Nq, a.d,
+                               p.splits, rows * a.d);
+            AADG_LAUNCH_CHECK();
+        }
+    }
+    return 0;
+}
+
+size_t at_delta_bytes(const aadg_attention_desc* s) { return aadg_align_up((size_t)s->B * s->H * s->Nq * 4, 256); }
+
+}  // namespace
+
+extern "C" int aadg_attention_supported(const aadg_attention_desc* desc_host) { return at_check(desc_host) == 0 ? 1 : 0; }
+
+extern "C" size_t aadg_attention_forward_workspace_bytes(const aadg_attention_desc* desc_host) {
+    return at_check(desc_host) == 0 ? at_fwd_bytes(desc_host) : 0;
+}
+
+extern "C" size_t aadg_attention_backward_workspace_bytes(const aadg_attention_desc* desc_host) {
+    if (at_check(desc_host) != 0) return 0;
+    const AtPlan pk = at_plan_keys(desc_host), pq = at_plan_rows(desc_host);
+    const size_t row = (size_t)desc_host->d * 4;
+    const size_t nk = pk.splits > 1 ? (size_t)pk.splits * 2 * desc_host->B * desc_host->G * desc_host->Nk * row : 0;
+    const size_t nq = pq.splits > 1 ? (size_t)pq.splits * desc_host->B * desc_host->H * desc_host->Nq * row : 0;
+    return at_delta_bytes(desc_host) + (nk > nq ? nk : nq);          // dk / dv are joined before dq reuses the partials
+}
+
+extern "C" int aadg_attention_forward(const aadg_attention_desc* desc_host, const void* q, const void* k, const void* v, const int* key_lengths,
+                                      void* o, float* lse, void* ws, size_t ws_bytes, void* stream) {
+    const int rc = at_check(desc_host);
+    if (rc != 0) return rc;
+    if (!at_aligned(desc_host, q, desc_host->q_stride) || !at_aligned(desc_host, k, desc_host->k_stride) ||
+        !at_aligned(desc_host, v, desc_host->v_stride) || !at_aligned(desc_host, o, desc_host->o_stride)) return AADG_E_BADARG;
+    const size_t need = at_fwd_bytes(desc_host);
+    if (need > 0 && (ws == nullptr || (uintptr_t)ws % 16 != 0 || ws_bytes < need)) return AADG_E_WORKSPACE;
+    AtArgs a = {};
+    at_fill(a, desc_host, key_lengths);
+    a.q = q; a.k = k; a.v = v; a.out = o; a.lse = lse;
+    const AtPlan p = at_plan_rows(desc_host);
+    a.part = (float*)ws;
+    a.ml = a.part + (size_t)p.splits * a.B * a.H * a.Nq * a.d;
+    return desc_host->dtype == 1 ? at_forward<uint16_t>(a, p, (hipStream_t)stream) : at_forward<float>(a, p, (hipStream_t)stream);
+}
+
+extern "C" int aadg_attention_backward(const aadg_attention_desc* desc_host, const void* q, const void* k, const void* v, const int* key_lengths,
+                                       const void* o, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
+                                       size_t ws_bytes, void* stream) {
+    const int rc = at_check(desc_host);
+    if (rc != 0) return rc;
+    if (!at_aligned(desc_host, q, desc_host->q_stride) || !at_aligned(desc_host, k, desc_host->k_stride) ||
+        !at_aligned(desc_host, v, desc_host->v_stride) || !at_aligned(desc_host, o, desc_host->o_stride) ||
+        !at_aligned(desc_host, dout, desc_host->do_stride) || lse == nullptr || (dk == nullptr) != (dv == nullptr)) return AADG_E_BADARG;
+    if (dq != nullptr && !at_aligned(desc_host, dq, desc_host->dq_stride)) return AADG_E_BADARG;
+    if (dk != nullptr && (!at_aligned(desc_host, dk, desc_host->dk_stride) || !at_aligned(desc_host, dv, desc_host->dv_stride))) return AADG_E_BADARG;
+    if (dq == nullptr && dk == nullptr) return 0;
+    if (ws == nullptr || (uintptr_t)ws % 16 != 0 || ws_bytes < aadg_attention_backward_workspace_bytes(desc_host)) return AADG_E_WORKSPACE;
+    AtArgs a = {};
+    at_fill(a, desc_host, key_lengths);
+    a.q = q; a.k = k; a.v = v; a.o = o; a.lse = const_cast<float*>(lse); a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
+    a.delta = (float*)ws;
+    a.part = (float*)((char*)ws + at_delta_bytes(desc_host));
+    return desc_host->dtype == 1 ? at_backward<uint16_t>(a, desc_host, (hipStream_t)stream) : at_backward<float>(a, desc_host, (hipStream_t)stream);
+}

@@ -630,6 +630,33 @@ int aadg_upsample_sum_backward_all_supported(int H, int W, const int* low_h, con
 int aadg_upsample_sum_backward_all(const void* dout, void* const* dlows, const int* low_h, const int* low_w, int n_low, int planes,
                                    int H, int W, int dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Softmax attention and its gradient (reference: models/mmseg/models/backbones/mix_transformer.py:86-100).
+ *   q, o [B, H, Nq, d], k, v [B, G, Nk, d], H % G == 0: head h reads key head h / (H / G).  dtype 0 float32 / 1 bfloat16 for all tensors.
+ *   s_ij = scale q_i . k_j;   key j is seen by query i of sequence b iff j < L_b and (causal == 0 or j <= i + L_b - Nq), with
+ *   L_b = key_lengths[b] clamped to 0 .. Nk (key_lengths NULL: Nk);   o_i = sum_j softmax_j(s_ij) v_j, 0 where no key is seen.
+ * Strides are in elements, for (batch, head, row); the d values of a row are contiguous.  d % 8 == 0, d <= 128; every pointer and
+ * stride a multiple of 16 bytes; 0 < scale < inf.  Keys and values behind L_b are never used.  lse [B, H, Nq] float32: log2 of the
+ * softmax denominators (+inf for a row without keys), written by the forward (NULL: not), read by the backward.
+ * Backward: from dout [B, H, Nq, d] dq, dk, dv (dq NULL, or dk and dv NULL: not computed); dk / dv are summed over the heads that
+ * share a key head and are zero behind L_b.  Sums have a fixed order: equal inputs give equal bits.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct aadg_attention_desc {
+    int32_t dtype, B, H, G, Nq, Nk, d, causal;
+    float scale;
+    int32_t reserved;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+    int64_t do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];      /* backward only */
+} aadg_attention_desc;
+int aadg_attention_supported(const aadg_attention_desc* desc_host);
+size_t aadg_attention_forward_workspace_bytes(const aadg_attention_desc* desc_host);
+int aadg_attention_forward(const aadg_attention_desc* desc_host, const void* q, const void* k, const void* v, const int* key_lengths,
+                           void* o, float* lse, void* ws, size_t ws_bytes, void* stream);
+size_t aadg_attention_backward_workspace_bytes(const aadg_attention_desc* desc_host);
+int aadg_attention_backward(const aadg_attention_desc* desc_host, const void* q, const void* k, const void* v, const int* key_lengths,
+                            const void* o, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
+                            size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

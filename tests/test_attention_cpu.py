@@ -1,0 +1,58 @@
+"""CPU: the attention entry points check their arguments on the host, before anything touches a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+
+def _desc(_lib, **kw):
+    d = _lib._AttentionDesc()
+    for k, v in dict(dtype=1, B=2, H=4, G=2, Nq=8, Nk=16, d=64, causal=0, scale=0.125).items():
+        setattr(d, k, kw.pop(k, v))
+    for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv"):
+        setattr(d, n + "_stride", (ctypes.c_int64 * 3)(*kw.pop(n, (4096, 512, 64))))
+    assert not kw
+    return d
+
+
+def test_attention_entry_points_validate_arguments():
+    from aadg_amd import _lib
+    lib = _lib.load()
+    z, one, odd = ctypes.c_void_p(0), ctypes.c_void_p(16), ctypes.c_void_p(24)
+    ref = ctypes.byref
+    ok = _desc(_lib)
+    assert lib.aadg_attention_supported(ref(ok)) == 1 and lib.aadg_attention_supported(z) == 0
+    for kw, rc in ((dict(dtype=2), -1), (dict(B=0), -1), (dict(Nq=0), -1), (dict(Nk=0), -1), (dict(G=3), -1), (dict(scale=0.0), -1), (dict(scale=-1.0), -1),
+                   (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(d=60), -3), (dict(d=136), -3), (dict(Nk=1 << 31 - 1), -3),
+                   (dict(B=1 << 20), -3)):
+        d = _desc(_lib, **kw)
+        assert lib.aadg_attention_supported(ref(d)) == 0, kw
+        assert lib.aadg_attention_forward(ref(d), one, one, one, z, one, z, z, 0, z) == rc, kw
+        assert lib.aadg_attention_backward(ref(d), one, one, one, z, one, one, one, one, one, one, one, 1 << 40, z) == rc, kw
+        assert lib.aadg_attention_forward_workspace_bytes(ref(d)) == 0 and lib.aadg_attention_backward_workspace_bytes(ref(d)) == 0
+    # pointers and strides: NULL, not on a 16-byte boundary
+    for args in ((z, one, one, one), (one, z, one, one), (one, one, z, one), (one, one, one, z), (odd, one, one, one)):
+        q, k, v, o = args
+        assert lib.aadg_attention_forward(ref(ok), q, k, v, z, o, z, z, 0, z) == -1
+        assert lib.aadg_attention_backward(ref(ok), q, k, v, z, o, one, one, one, one, one, one, 1 << 40, z) == -1
+    assert lib.aadg_attention_forward(ref(_desc(_lib, k=(4096, 512, 60))), one, one, one, z, one, z, z, 0, z) == -1
+    assert lib.aadg_attention_backward(ref(ok), one, one, one, z, one, z, one, one, one, one, one, 1 << 40, z) == -1          # no lse
+    assert lib.aadg_attention_backward(ref(ok), one, one, one, z, one, one, one, one, one, z, one, 1 << 40, z) == -1          # dk without dv
+    assert lib.aadg_attention_backward(ref(_desc(_lib, dv=(4096, 512, 4))), one, one, one, z, one, one, one, one, one, one, one, 1 << 40, z) == -1
+    # workspaces
+    assert lib.aadg_attention_backward(ref(ok), one, one, one, z, one, one, one, one, one, one, one, 16, z) == -2
+    long = _desc(_lib, B=1, Nq=1, Nk=4096)
+    need = lib.aadg_attention_forward_workspace_bytes(ref(long))
+    assert need > 0
+    assert lib.aadg_attention_forward(ref(long), one, one, one, z, one, z, one, need - 1, z) == -2
+    assert lib.aadg_attention_forward(ref(long), one, one, one, z, one, z, z, need, z) == -2
+    assert lib.aadg_attention_backward(ref(ok), one, one, one, z, one, one, one, z, z, z, z, 0, z) == 0                        # nothing asked for
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU behaviour")
+def test_attention_has_no_cpu_path():
+    from aadg_amd import _lib
+    q = torch.zeros(1, 1, 4, 64)
+    assert not _lib.attention_supported(q, q, q)
+    with pytest.raises(_lib.AadgError):
+        _lib.attention(q, q, q)
