@@ -4,7 +4,7 @@ torch is used only as plumbing here: device memory, the current HIP stream, and 
 There is deliberately NO CPU fallback: every wrapper raises if the shared library or a GPU is
 missing, so a silent eager path can never stand in for the HIP kernels.
 
-One namespace, nine modules by concern (round 6; it was one 2.9 k-line file):
+One namespace, ten modules by concern (round 6; it was one 2.9 k-line file):
 
     binding    the loader, the symbol table, errors, stream / pointer / workspace helpers
     aug        the fused uint8 augmentation call and its planner statement
@@ -15,6 +15,7 @@ One namespace, nine modules by concern (round 6; it was one 2.9 k-line file):
     weights    bfloat16 / split shadows of the master weights
     conv       the matrix-core convolutions (bfloat16 and f32x3)
     attn       softmax attention, forward and backward
+    ortho      orthogonalised matrix updates (the Muon optimiser's operator)
 
 `from aadg_amd import _lib; _lib.<anything>` keeps working: every name of every module is re-exported here, and an ASSIGNMENT through this
 namespace (`_lib.BN_SYNC_REDUCE = f`, `_lib.PROFILE_EVENTS = pair`, a test's `monkeypatch.setattr(_lib, "conv1x1", g)`) is forwarded to
@@ -28,9 +29,9 @@ import types
 import numpy as np
 import torch
 
-from . import binding, aug, hotpath, layers, batchnorm, wgrad, weights, conv, attn
+from . import binding, aug, hotpath, layers, batchnorm, wgrad, weights, conv, attn, ortho
 
-_MODULES = (binding, aug, hotpath, layers, batchnorm, wgrad, weights, conv, attn)
+_MODULES = (binding, aug, hotpath, layers, batchnorm, wgrad, weights, conv, attn, ortho)
 
 for _m in _MODULES:
     for _k, _v in vars(_m).items():

@@ -62,6 +62,7 @@ EXPORTS = [
     "aadg_bn_sync_backward_res_bn_f32", "aadg_draw_python_stream",
     "aadg_attention_supported", "aadg_attention_forward_workspace_bytes", "aadg_attention_forward",
     "aadg_attention_backward_workspace_bytes", "aadg_attention_backward",
+    "aadg_orthogonalize_workspace_bytes", "aadg_orthogonalize_f32",
 ]
 
 _lib = None
@@ -304,6 +305,10 @@ def load():
     lib.aadg_attention_backward_workspace_bytes.argtypes = [_vp]
     lib.aadg_attention_backward.restype = _i
     lib.aadg_attention_backward.argtypes = [_vp] * 12 + [_sz, _vp]
+    lib.aadg_orthogonalize_workspace_bytes.restype = _sz
+    lib.aadg_orthogonalize_workspace_bytes.argtypes = [_vp, _i]
+    lib.aadg_orthogonalize_f32.restype = _i
+    lib.aadg_orthogonalize_f32.argtypes = [_vp, _i, _i, _f, _f, _f, _f, _vp, _sz, _vp]
     if lib.aadg_abi_version() != 12:
         raise RuntimeError("libaadg_hip.so ABI version mismatch")
     _lib = lib

@@ -1,0 +1,388 @@
+// Orthogonalised updates: a list of float32 matrices U is replaced by an odd polynomial of each that moves its singular values towards
+// one (Newton-Schulz iteration with the quintic the Muon optimiser uses), for the trained matrices of the segmentation networks.
+//
+//   X = U / (|U|_F + eps);   steps times:   A = X X^T,   B = b A + c A A,   X <- a X + B X          (X [m, n], m <= n: U or U^T)
+//
+// Flops per step: m^2 n + m^3 (two symmetric products, one triangle each) + 2 m^2 n.
+// The iteration magnifies small singular values by a per step, and with them whatever error the products leave (bfloat16 products: 1e-2 of
+// the result after five steps, products of two bfloat16 halves 4e-5, float32 3e-6), so the products are float32-grade: every operand
+// is kept as THREE bfloat16 planes, x = x0 + x1 + x2 (24 significant bits), and a product is the six plane products of weight 2^-16 or
+// more, summed in float32 on the bfloat16 matrix cores -- six at 16 times the rate of the float32 matrix instructions.  The planes are
+// written by the kernel that produces a matrix, once per element; the product kernels move bfloat16 only.
+//
+// All matrices of the list go through each phase in ONE launch: a workgroup finds its matrix from the running tile counts of a table in the
+// workspace.  The table travels in kernel arguments (32 entries a launch), so a captured graph keeps it.
+#include "common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 or_bf16x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef short or_v4i16 __attribute__((ext_vector_type(4)));
+typedef short or_v8i16 __attribute__((ext_vector_type(8)));
+typedef uint32_t or_u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int OR_BK = 32;                             // contracted values per LDS stage
+constexpr int OR_SUM = 16384;                         // elements per workgroup of the norm
+constexpr int OR_CHUNK = 32;                          // table entries per launch (kernel arguments: 4 KB)
+
+enum { OR_P_SUM, OR_P_SPLIT, OR_P_SYM, OR_P_X, OR_PHASES };
+
+struct OrMat {
+    const float* src;
+    float* dst;
+    long long x0, x1, a, b, sums;                     // byte offsets of the planes and the partial sums in the workspace
+    int rows, cols, m, n, ldx, lda;
+    int first[OR_PHASES];                             // index of the matrix's first workgroup in each phase
+    int pad;
+};
+struct OrChunk { OrMat mat[OR_CHUNK]; int base, count; };
+
+__global__ void k_or_table(const OrChunk c, OrMat* __restrict__ table) {
+    const int words = c.count * (int)(sizeof(OrMat) / 4);
+    const int* s = reinterpret_cast<const int*>(c.mat);
+    int* d = reinterpret_cast<int*>(table + c.base);
+    for (int i = threadIdx.x; i < words; i += blockDim.x) d[i] = s[i];
+}
+
+// the matrix workgroup `wg` of phase `ph` belongs to: the last one whose first workgroup is not behind it (one wave, 64 entries at a time)
+__device__ __forceinline__ int or_find(const OrMat* __restrict__ table, int count, int ph, int wg) {
+    int at = -1;
+    for (int base = 0; base < count; base += 64) {
+        const int i = base + (threadIdx.x & 63);
+        const bool le = i < count && table[i].first[ph] <= wg;
+        const unsigned long long mask = __ballot(le);
+        at += __popcll(mask);
+        if (mask != ~0ull) break;
+    }
+    return __builtin_amdgcn_readfirstlane(at);
+}
+
+__device__ __forceinline__ void or_split(float x, uint16_t* p) {
+    const uint32_t h = aadg_f2bf_bits(x);
+    const float r = x - __uint_as_float(h << 16);
+    const uint32_t g = aadg_f2bf_bits(r);
+    p[0] = (uint16_t)h;
+    p[1] = (uint16_t)g;
+    p[2] = (uint16_t)aadg_f2bf_bits(r - __uint_as_float(g << 16));
+}
+__device__ __forceinline__ float or_join(uint16_t a, uint16_t b, uint16_t c) {
+    return __uint_as_float((uint32_t)a << 16) + (__uint_as_float((uint32_t)b << 16) + __uint_as_float((uint32_t)c << 16));
+}
+
+// partial sums of squares in double (squares of small gradients leave float32's range), OR_SUM elements a workgroup
+__global__ __launch_bounds__(256) void k_or_sum(const OrMat* __restrict__ table, int count, char* __restrict__ ws) {
+    __shared__ double part[4];
+    const OrMat& t = table[or_find(table, count, OR_P_SUM, blockIdx.x)];
+    const int w = blockIdx.x - t.first[OR_P_SUM];
+    const long long total = (long long)t.rows * t.cols, lo = (long long)w * OR_SUM, hi = min(total, lo + OR_SUM);
+    double s = 0.0;
+    for (long long i = lo + threadIdx.x; i < hi; i += 256) {
+        const double x = t.src[i];
+        s = fma(x, x, s);
+    }
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) reinterpret_cast<double*>(ws + t.sums)[w] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// X = U / (|U| + eps) as planes, 32 x 32 elements a workgroup, transposed through LDS where U is tall
+__global__ __launch_bounds__(256) void k_or_planes(const OrMat* __restrict__ table, int count, char* __restrict__ ws, float eps) {
+    __shared__ float tile[32][33];
+    __shared__ float scale_s;
+    const OrMat& t = table[or_find(table, count, OR_P_SPLIT, blockIdx.x)];
+    const int w = blockIdx.x - t.first[OR_P_SPLIT], tn = (t.ldx + 31) / 32;
+    const int r0 = w / tn * 32, c0 = (w - w / tn * tn) * 32;
+    if (threadIdx.x < 64) {
+        const int parts = (int)(((long long)t.rows * t.cols + OR_SUM - 1) / OR_SUM);
+        const double* p = reinterpret_cast<const double*>(ws + t.sums);
+        double s = 0.0;
+        for (int i = threadIdx.x; i < parts; i += 64) s += p[i];
+        s = wave_sum(s);
+        if (threadIdx.x == 0) scale_s = (float)(1.0 / (sqrt(s) + (double)eps));
+    }
+    const bool tall = t.rows > t.cols;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int y = ty + 8 * i;
+        // X[r0 + y][c0 + tx] = U[..][..]; tall: U[c0 + y][r0 + tx] = X[r0 + tx][c0 + y]
+        if (!tall) tile[y][tx] = r0 + y < t.m && c0 + tx < t.n ? t.src[(long long)(r0 + y) * t.cols + c0 + tx] : 0.0f;
+        else tile[tx][y] = c0 + y < t.n && r0 + tx < t.m ? t.src[(long long)(c0 + y) * t.cols + r0 + tx] : 0.0f;
+    }
+    __syncthreads();
+    const float scale = scale_s;
+    uint16_t* x = reinterpret_cast<uint16_t*>(ws + t.x0);
+    const long long plane = (long long)t.m * t.ldx;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + ty + 8 * i, c = c0 + tx;
+        if (r >= t.m || c >= t.ldx) continue;
+        uint16_t p[3];
+        or_split(tile[ty + 8 * i][tx] * scale, p);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) x[k * plane + (long long)r * t.ldx + c] = p[k];
+    }
+}
+
+// LDS layouts.  K-contiguous operand: rows of OR_BK values, chunk c of row r at c ^ ((r >> 2) & 3): 8 rows of one chunk hit all banks.
+__device__ __forceinline__ int or_row_at(int row, int chunk) { return row * OR_BK + ((chunk ^ ((row >> 2) & 3)) << 3); }
+// K-strided operand ([k][TB] as in memory): chunks permuted such that the 4 rows x 4 chunks of a transpose read hit all banks
+template <int TB> __device__ __forceinline__ int or_col_at(int k, int chunk) {
+    return k * TB + ((chunk ^ (TB == 128 ? ((k & 3) << 2) | ((k >> 2) & 3) : (((k >> 1) & 1) << 2) | ((k >> 2) & 3))) << 3);
+}
+template <int TB> __device__ __forceinline__ or_bf16x8 or_cols(const uint16_t* t, int k0, int c0, int lane) {
+    const int i = lane & 15, k = k0 + 8 * (lane >> 5) + (i >> 2), c = c0 + (lane & 16) + 4 * (i & 3);
+    typedef or_v4i16 __attribute__((address_space(3)))* lds_p;
+    const or_v4i16 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(t + or_col_at<TB>(k, c >> 3) + (c & 7)));
+    const or_v4i16 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(t + or_col_at<TB>(k + 4, c >> 3) + (c & 7)));
+    const or_v8i16 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return __builtin_bit_cast(or_bf16x8, v);
+}
+
+// One TB x TB tile of a product, 4 waves of (TB / 2) x (TB / 2).
+//   PH = OR_A: A = X X^T          (tiles i >= j, stored twice)
+//   PH = OR_B: B = b A + c A A    (A symmetric: A A^T; tiles i >= j, stored twice)
+//   PH = OR_X: X' = a X + B X     (the second operand K-strided: transpose reads); last step: to the caller's matrix instead
+enum { OR_A, OR_B, OR_X };
+template <int PH, int TB>
+__global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table, int count, char* __restrict__ ws, float ca, float cb, int odd, int last) {
+    constexpr int W = TB / 64, LR = 3 * TB * (OR_BK / 8) / 256;             // 32-wide blocks per wave side; 16-byte chunks per thread and operand
+    __shared__ __attribute__((aligned(16))) uint16_t Ls[3 * TB * OR_BK], Rs[3 * TB * OR_BK];
+    const OrMat t = table[or_find(table, count, PH == OR_X ? OR_P_X : OR_P_SYM, blockIdx.x)];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    int w = blockIdx.x - t.first[PH == OR_X ? OR_P_X : OR_P_SYM], ti, tj;
+    if (PH == OR_X) {
+        const int tn = (t.ldx + TB - 1) / TB;
+        ti = w / tn;
+        tj = w - ti * tn;
+    } else {                                                               // w = ti (ti + 1) / 2 + tj, tj <= ti
+        ti = (int)((sqrtf(8.0f * w + 1.0f) - 1.0f) * 0.5f);
+        while (ti * (ti + 1) / 2 > w) --ti;
+        while ((ti + 1) * (ti + 2) / 2 <= w) ++ti;
+        tj = w - ti * (ti + 1) / 2;
+    }
+    const uint16_t* X = reinterpret_cast<const uint16_t*>(ws + (odd ? t.x1 : t.x0));
+    const uint16_t* L = PH == OR_A ? X : reinterpret_cast<const uint16_t*>(ws + (PH == OR_B ? t.a : t.b));
+    const uint16_t* R = PH == OR_B ? L : X;
+    const int ldl = PH == OR_A ? t.ldx : t.lda, ldr = PH == OR_B ? t.lda : t.ldx, K = PH == OR_A ? t.ldx : t.lda;
+    const long long pl_l = (long long)t.m * ldl, pl_r = (long long)t.m * ldr;
+    const int i0 = ti * TB, j0 = tj * TB, wi = (wv >> 1) * (TB / 2), wj = (wv & 1) * (TB / 2);
+
+    uint4 rl[LR], rr[LR];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LR; ++i) {
+            const int id = tid + 256 * i;
+            {
+                const int pl = id / (TB * 4), q = id - pl * (TB * 4), row = i0 + (q >> 2), k = k0 + (q & 3) * 8;
+                const uint4 x = *reinterpret_cast<const uint4*>(L + pl * pl_l + (long long)min(row, t.m - 1) * ldl + min(k, ldl - 8));
+                rl[i] = row < t.m && k < ldl ? x : make_uint4(0, 0, 0, 0);
+            }
+            if (PH != OR_X) {
+                const int pl = id / (TB * 4), q = id - pl * (TB * 4), row = j0 + (q >> 2), k = k0 + (q & 3) * 8;
+                const uint4 x = *reinterpret_cast<const uint4*>(R + pl * pl_r + (long long)min(row, t.m - 1) * ldr + min(k, ldr - 8));
+                rr[i] = row < t.m && k < ldr ? x : make_uint4(0, 0, 0, 0);
+            } else {
+                const int pl = id / (OR_BK * (TB / 8)), q = id - pl * (OR_BK * (TB / 8)), k = k0 + q / (TB / 8), c = j0 + (q % (TB / 8)) * 8;
+                const uint4 x = *reinterpret_cast<const uint4*>(R + pl * pl_r + (long long)min(k, t.m - 1) * ldr + min(c, ldr - 8));
+                rr[i] = k < t.m && c < ldr ? x : make_uint4(0, 0, 0, 0);
+            }
+        }
+    };
+    f32x16 acc[W][W];
+#pragma unroll
+    for (int x = 0; x < W; ++x)
+#pragma unroll
+        for (int y = 0; y < W; ++y)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[x][y][i] = 0.0f;
+    fetch(0);
+    for (int k0 = 0; k0 < K; k0 += OR_BK) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LR; ++i) {
+            const int id = tid + 256 * i;
+            {
+                const int pl = id / (TB * 4), q = id - pl * (TB * 4);
+                *reinterpret_cast<uint4*>(&Ls[pl * TB * OR_BK + or_row_at(q >> 2, q & 3)]) = rl[i];
+                if (PH != OR_X) *reinterpret_cast<uint4*>(&Rs[pl * TB * OR_BK + or_row_at(q >> 2, q & 3)]) = rr[i];
+            }
+            if (PH == OR_X) {
+                const int pl = id / (OR_BK * (TB / 8)), q = id - pl * (OR_BK * (TB / 8));
+                *reinterpret_cast<uint4*>(&Rs[pl * TB * OR_BK + or_col_at<TB>(q / (TB / 8), q % (TB / 8))]) = rr[i];
+            }
+        }
+        __syncthreads();
+        if (k0 + OR_BK < K) fetch(k0 + OR_BK);
+#pragma unroll
+        for (int u = 0; u < OR_BK / 16; ++u) {
+            or_bf16x8 l[3][W], r[3][W];
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+#pragma unroll
+                for (int x = 0; x < W; ++x) {
+                    l[p][x] = __builtin_bit_cast(or_bf16x8, *reinterpret_cast<const or_u32x4*>(&Ls[p * TB * OR_BK + or_row_at(wi + 32 * x + (lane & 31), 2 * u + h)]));
+                    if (PH != OR_X)
+                        r[p][x] = __builtin_bit_cast(or_bf16x8, *reinterpret_cast<const or_u32x4*>(&Rs[p * TB * OR_BK + or_row_at(wj + 32 * x + (lane & 31), 2 * u + h)]));
+                    else
+                        r[p][x] = or_cols<TB>(&Rs[p * TB * OR_BK], 16 * u, wj + 32 * x, lane);
+                }
+            // weights 2^-16, 2^-8, 1: the small ones first.  The six start from zero and their sum is added to the accumulator by the vector
+            // unit: accumulating in the matrix instruction rounds 6 K / 16 times at the size of the whole sum and with a bias (3.7e-6
+            // instead of 6e-7 of the result at K = 768)
+#pragma unroll
+            for (int x = 0; x < W; ++x)
+#pragma unroll
+                for (int y = 0; y < W; ++y) {
+                    f32x16 d = {};
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[2][x], r[0][y], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[2][y], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[1][x], r[1][y], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[1][x], r[0][y], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[1][y], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[0][y], d, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[x][y][i] += d[i];
+                }
+        }
+    }
+    // epilogue: register i of half h = row 8 (i / 4) + 4 h + i % 4, lane & 31 = column
+    uint16_t* out = reinterpret_cast<uint16_t*>(ws + (PH == OR_A ? t.a : PH == OR_B ? t.b : odd ? t.x0 : t.x1));
+    const int ldo = PH == OR_X ? t.ldx : t.lda;
+    const long long pl_o = (long long)t.m * ldo;
+    const bool tall = t.rows > t.cols;
+#pragma unroll
+    for (int x = 0; x < W; ++x)
+#pragma unroll
+        for (int y = 0; y < W; ++y) {
+            const int col = j0 + wj + 32 * y + (lane & 31);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = i0 + wi + 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
+                float v = acc[x][y][i];
+                if (PH == OR_X) {
+                    if (row >= t.m || col >= t.ldx) continue;
+                    const long long e = (long long)row * ldo + col;
+                    v = fmaf(ca, or_join(X[e], X[pl_o + e], X[2 * pl_o + e]), v);
+                    if (last) {
+                        if (col < t.n) t.dst[tall ? (long long)col * t.cols + row : (long long)row * t.cols + col] = v;
+                        continue;
+                    }
+                    uint16_t p[3];
+                    or_split(v, p);
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) out[k * pl_o + e] = p[k];
+                } else {
+                    const long long e = (long long)row * ldo + col, f = (long long)col * ldo + row;
+                    const bool in = row < t.m && col < t.lda, mirror = ti != tj && col < t.m && row < t.lda;
+                    if (PH == OR_B) {
+                        const bool have = row < t.m && col < t.m;
+                        v = have ? fmaf(cb, v, ca * or_join(L[e], L[pl_o + e], L[2 * pl_o + e])) : 0.0f;
+                    }
+                    uint16_t p[3];
+                    or_split(v, p);
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        if (in) out[k * pl_o + e] = p[k];
+                        if (mirror) out[k * pl_o + f] = p[k];
+                    }
+                }
+            }
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+constexpr int OR_MAX_SIDE = 1 << 16, OR_MAX_MATS = 4096;
+
+struct OrLayout { size_t bytes; long long grid[OR_PHASES]; int tb; };
+
+// 0 or an error; fills the entries if `out` is given (n entries)
+int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out) {
+    if (mats == nullptr || n < 1 || n > OR_MAX_MATS) return AADG_E_BADARG;
+    for (int i = 0; i < n; ++i) {
+        if (mats[i].rows < 1 || mats[i].cols < 1) return AADG_E_BADARG;
+        if (mats[i].rows > OR_MAX_SIDE || mats[i].cols > OR_MAX_SIDE || (long long)mats[i].rows * mats[i].cols > (1 << 28)) return AADG_E_UNSUPPORTED;
+    }
+    long long big = 0;
+    for (int i = 0; i < n; ++i) {
+        const long long m = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, k = (m + 127) / 128;
+        big += k * (k + 1) / 2;
+    }
+    lay.tb = big >= 256 ? 128 : 64;                   // fewer 128-wide tiles in the smallest phase than CUs: 64
+    size_t at = aadg_align_up((size_t)n * sizeof(OrMat), 256);
+    for (int p = 0; p < OR_PHASES; ++p) lay.grid[p] = 0;
+    for (int i = 0; i < n; ++i) {
+        OrMat t = {};
+        t.src = mats[i].src; t.dst = mats[i].dst; t.rows = mats[i].rows; t.cols = mats[i].cols;
+        t.m = t.rows < t.cols ? t.rows : t.cols;
+        t.n = t.rows < t.cols ? t.cols : t.rows;
+        t.ldx = (t.n + 7) / 8 * 8;
+        t.lda = (t.m + 7) / 8 * 8;
+        const size_t px = aadg_align_up((size_t)3 * t.m * t.ldx * 2, 256), pa = aadg_align_up((size_t)3 * t.m * t.lda * 2, 256);
+        const long long parts = ((long long)t.rows * t.cols + OR_SUM - 1) / OR_SUM, tm = (t.m + lay.tb - 1) / lay.tb, tn = (t.ldx + lay.tb - 1) / lay.tb;
+        t.x0 = (long long)at; at += px;
+        t.x1 = (long long)at; at += px;
+        t.a = (long long)at; at += pa;
+        t.b = (long long)at; at += pa;
+        t.sums = (long long)at; at += aadg_align_up((size_t)parts * 8, 256);
+        const long long wgs[OR_PHASES] = {parts, (long long)((t.m + 31) / 32) * ((t.ldx + 31) / 32), tm * (tm + 1) / 2, tm * tn};
+        for (int p = 0; p < OR_PHASES; ++p) {
+            t.first[p] = (int)lay.grid[p];
+            lay.grid[p] += wgs[p];
+            if (lay.grid[p] > 0x7FFFFFFF) return AADG_E_UNSUPPORTED;
+        }
+        if (out != nullptr) out[i] = t;
+    }
+    lay.bytes = at;
+    return 0;
+}
+
+template <int TB> int or_steps(const OrLayout& lay, const OrMat* table, int n, int steps, float a, float b, float c, char* ws, hipStream_t st) {
+    for (int s = 0; s < steps; ++s) {
+        hipLaunchKernelGGL((k_or_mul<OR_A, TB>), dim3((unsigned)lay.grid[OR_P_SYM]), dim3(256), 0, st, table, n, ws, 0.0f, 0.0f, s & 1, 0);
+        hipLaunchKernelGGL((k_or_mul<OR_B, TB>), dim3((unsigned)lay.grid[OR_P_SYM]), dim3(256), 0, st, table, n, ws, b, c, s & 1, 0);
+        hipLaunchKernelGGL((k_or_mul<OR_X, TB>), dim3((unsigned)lay.grid[OR_P_X]), dim3(256), 0, st, table, n, ws, a, 0.0f, s & 1, s == steps - 1);
+        AADG_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" size_t aadg_orthogonalize_workspace_bytes(const aadg_matrix* mats_host, int n) {
+    OrLayout lay;
+    return or_layout(mats_host, n, lay, nullptr) == 0 ? lay.bytes : 0;
+}
+
+extern "C" int aadg_orthogonalize_f32(const aadg_matrix* mats_host, int n, int steps, float a, float b, float c, float eps, void* ws,
+                                      size_t ws_bytes, void* stream) {
+    OrLayout lay;
+    const int rc = or_layout(mats_host, n, lay, nullptr);
+    if (rc != 0) return rc;
+    if (steps < 1 || steps > 64 || !(eps >= 0.0f)) return AADG_E_BADARG;
+    for (int i = 0; i < n; ++i)
+        if (mats_host[i].src == nullptr || mats_host[i].dst == nullptr || (uintptr_t)mats_host[i].src % 4 != 0 || (uintptr_t)mats_host[i].dst % 4 != 0)
+            return AADG_E_BADARG;
+    if (ws == nullptr || (uintptr_t)ws % 256 != 0 || ws_bytes < lay.bytes) return AADG_E_WORKSPACE;
+    OrMat* entries = (OrMat*)malloc((size_t)n * sizeof(OrMat));
+    if (entries == nullptr) return AADG_E_WORKSPACE;
+    or_layout(mats_host, n, lay, entries);
+    hipStream_t st = (hipStream_t)stream;
+    OrMat* table = (OrMat*)ws;
+    constexpr int PER = OR_CHUNK;
+    static_assert(sizeof(OrChunk) + sizeof(OrMat*) <= 4096, "kernel arguments");
+    for (int i = 0; i < n; i += PER) {
+        OrChunk chunk = {};
+        chunk.base = i;
+        chunk.count = n - i < PER ? n - i : PER;
+        memcpy(chunk.mat, entries + i, (size_t)chunk.count * sizeof(OrMat));
+        hipLaunchKernelGGL(k_or_table, dim3(1), dim3(256), 0, st, chunk, table);
+    }
+    free(entries);
+    hipLaunchKernelGGL(k_or_sum, dim3((unsigned)lay.grid[OR_P_SUM]), dim3(256), 0, st, table, n, (char*)ws);
+    hipLaunchKernelGGL(k_or_planes, dim3((unsigned)lay.grid[OR_P_SPLIT]), dim3(256), 0, st, table, n, (char*)ws, eps);
+    AADG_LAUNCH_CHECK();
+    return lay.tb == 128 ? or_steps<128>(lay, table, n, steps, a, b, c, (char*)ws, st) : or_steps<64>(lay, table, n, steps, a, b, c, (char*)ws, st);
+}

@@ -657,6 +657,21 @@ int aadg_attention_backward(const aadg_attention_desc* desc_host, const void* q,
                             const void* o, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
                             size_t ws_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Orthogonalised updates: dst = p(src / (|src|_F + eps)) for every matrix of a list, p = `steps` applications of the odd polynomial
+ * x -> a x + b x^3 + c x^5 to the singular values (x^3 = x x^T x).  float32, row-major, contiguous, any size up to 65536 a side and
+ * 2^28 elements, at most 4096 matrices; dst == src is allowed, other overlaps are not.  Products at float32 accuracy, sums in a fixed
+ * order.  The list (mats_host) is read during the call only.  ws: 256-byte aligned.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct aadg_matrix {
+    const float* src;
+    float* dst;
+    int32_t rows, cols;
+} aadg_matrix;
+size_t aadg_orthogonalize_workspace_bytes(const aadg_matrix* mats_host, int n);
+int aadg_orthogonalize_f32(const aadg_matrix* mats_host, int n, int steps, float a, float b, float c, float eps, void* ws,
+                           size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
