@@ -90,6 +90,15 @@ def _ln(norm, x, r=None, rscale=None):
     return x, norm(x)
 
 
+def _attend(q, k, v, scale):
+    """softmax(scale q k^T) v; on the GPU the own kernels (csrc/attention.hip), which read the projections' layouts in place"""
+    if q.is_cuda:
+        from .. import _lib
+        if _lib.attention_supported(q, k, v):
+            return _lib.attention(q, k, v, scale=scale)
+    return F.scaled_dot_product_attention(q, k, v, scale=scale)
+
+
 def _tokens_as_map(x, H, W):
     """[B, H*W, C] tokens viewed as a [B, C, H, W] tensor in channels-last memory format: no copy."""
     B, N, C = x.shape
@@ -162,8 +171,8 @@ class Attention(nn.Module):
             r = _ln(self.norm, r.flatten(2).transpose(1, 2))[1]
         else:
             r = x
-        kv = self.kv(r).view(B, -1, 2, h, d).permute(2, 0, 3, 1, 4)                      # [2, B, h, N', d]
-        o = F.scaled_dot_product_attention(q, kv[0], kv[1], scale=self.scale)            # softmax(q k^T * scale) v
+        k, v = self.kv(r).view(B, -1, 2, h, d).permute(2, 0, 3, 1, 4).unbind(0)          # [B, h, N', d] each
+        o = _attend(q, k, v, self.scale)                                                 # softmax(q k^T * scale) v
         return self.proj(o.transpose(1, 2).reshape(B, N, C))
 
 

@@ -1,0 +1,82 @@
+"""Muon: momentum whose update is orthogonalised, for the weight matrices of the segmentation networks; Adam for everything else.
+
+For a matrix parameter W (a convolution weight is the matrix [out, in * kh * kw]) with gradient G:
+    M <- momentum M + (1 - momentum) G          U = (1 - momentum) G + momentum M   (Nesterov)
+    W <- (1 - lr wd) W - lr 0.2 sqrt(max(rows, cols)) orthogonalize(U)
+The factor gives the update the root mean square of an Adam update (an orthogonal [m, n] matrix has 1 / sqrt(max(m, n))), so that one learning
+rate and its schedule serve both kinds of parameters.  The orthogonalisation of all matrices is one call (`_lib.orthogonalize`,
+csrc/orthogonalize.hip).  The reference trains with Adam only (scheduler.py:5-34); this is `run.py --optimizer muon`.
+"""
+import torch
+
+from . import _lib
+
+
+def is_matrix(p):
+    """Parameters the orthogonalised update is for: two or more axes, a filter over more than one input channel (depthwise filters are
+    vectors per channel) and at least 16 values along the shorter side (classifier rows and the like stay with Adam)."""
+    return p.dim() >= 2 and p.shape[1] > 1 and min(p.shape[0], p[0].numel()) >= 16
+
+
+class Muon(torch.optim.Optimizer):
+    """`params`: parameters on one GPU, split by `is_matrix` into a Muon and an Adam group (one learning rate, one decay).  `weight_decay` is
+    decoupled for the matrices and added to the gradient for the others, as in Adam.  Float32 parameters only."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.0, momentum=0.95, betas=(0.9, 0.999), eps=1e-8, steps=5):
+        params = [p for p in params if p.requires_grad]
+        for p in params:
+            if not p.is_cuda:
+                raise _lib.AadgError("Muon: parameters must be on the GPU (got %s); there is no CPU path" % p.device)
+            if p.dtype != torch.float32:
+                raise _lib.AadgError("Muon: float32 parameters only, got %s" % p.dtype)
+        if not lr >= 0.0 or not weight_decay >= 0.0 or not 0.0 <= momentum < 1.0 or not all(0.0 <= b < 1.0 for b in betas) or not eps > 0.0:
+            raise ValueError("Muon: lr %r, weight_decay %r, momentum %r, betas %r, eps %r" % (lr, weight_decay, momentum, betas, eps))
+        groups = [dict(params=[p for p in params if is_matrix(p)], matrices=True), dict(params=[p for p in params if not is_matrix(p)], matrices=False)]
+        super().__init__([g for g in groups if g["params"]],
+                         dict(lr=lr, weight_decay=weight_decay, momentum=momentum, betas=betas, eps=eps, steps=steps, matrices=True))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if params:
+                (self._matrices if group["matrices"] else self._others)(group, params, [p.grad for p in params])
+        return loss
+
+    def _matrices(self, group, params, grads):
+        for p in params:
+            if not self.state[p]:
+                self.state[p]["momentum"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+        bufs, mu, lr = [self.state[p]["momentum"] for p in params], group["momentum"], group["lr"]
+        torch._foreach_lerp_(bufs, grads, 1.0 - mu)
+        updates = torch._foreach_lerp(grads, bufs, mu)
+        flat = _lib.orthogonalize([u.reshape(u.shape[0], -1) for u in updates], steps=group["steps"])
+        out = [o.view(p.shape) for o, p in zip(flat, params)]
+        torch._foreach_mul_(out, [-0.2 * lr * max(o.shape) ** 0.5 for o in flat])
+        if group["weight_decay"] != 0.0:
+            torch._foreach_mul_(params, 1.0 - lr * group["weight_decay"])
+        torch._foreach_add_(params, out)
+
+    def _others(self, group, params, grads):
+        (b1, b2), lr, eps = group["betas"], group["lr"], group["eps"]
+        for p in params:
+            if not self.state[p]:
+                self.state[p].update(step=0, exp_avg=torch.zeros_like(p), exp_avg_sq=torch.zeros_like(p))
+        steps = []
+        for p in params:
+            self.state[p]["step"] += 1
+            steps.append(self.state[p]["step"])
+        m, v = [self.state[p]["exp_avg"] for p in params], [self.state[p]["exp_avg_sq"] for p in params]
+        if group["weight_decay"] != 0.0:
+            grads = torch._foreach_add(grads, params, alpha=group["weight_decay"])
+        torch._foreach_lerp_(m, grads, 1.0 - b1)
+        torch._foreach_mul_(v, b2)
+        torch._foreach_addcmul_(v, grads, grads, 1.0 - b2)
+        denom = torch._foreach_sqrt(v)
+        torch._foreach_div_(denom, [(1.0 - b2 ** s) ** 0.5 for s in steps])
+        torch._foreach_add_(denom, eps)
+        torch._foreach_addcdiv_(params, m, denom, [-lr / (1.0 - b1 ** s) for s in steps])

@@ -7,6 +7,8 @@ discriminator).  Function names and return tuples follow the reference."""
 from torch.optim import Adam
 from torch.optim.lr_scheduler import CosineAnnealingLR, MultiStepLR
 
+from .muon import Muon
+
 CONTROLLER_LR = 0.00035
 
 
@@ -32,9 +34,12 @@ def _model_adam(model, cfg):
     return _adam(model.parameters(), lr=cfg.TRAIN.LR, weight_decay=cfg.TRAIN.WD)
 
 
-def get_optimizer_scheduler(controller, model, cfg):
-    """-> (model optimiser, model LR scheduler, controller optimiser)"""
-    model_opt = _model_adam(model, cfg)
+def get_optimizer_scheduler(controller, model, cfg, optimizer='adam'):
+    """-> (model optimiser, model LR scheduler, controller optimiser); optimizer 'muon': orthogonalised updates of the weight matrices
+    (muon.py) under the same learning rate and schedule"""
+    if optimizer not in ('adam', 'muon'):
+        raise ValueError("optimizer: expected 'adam' or 'muon', got %r" % (optimizer,))
+    model_opt = Muon(model.parameters(), lr=cfg.TRAIN.LR, weight_decay=cfg.TRAIN.WD) if optimizer == 'muon' else _model_adam(model, cfg)
     return model_opt, _step_at_warmup_end(model_opt, cfg, 0.1), Adam(controller.parameters(), lr=CONTROLLER_LR)
 
 

@@ -254,7 +254,7 @@ class SearchState(object):
                 torch.distributed.broadcast(t.data, 0)             # once, at construction: the default group
         _, self.train_loader, self.test_loader = get_seg_dg_dataloader(config, args, self.batch_size, workers)
         self.model_optimizer, self.model_lrscheduler, self.controller_optimizer = \
-            get_optimizer_scheduler(self.controller, self.model, config)
+            get_optimizer_scheduler(self.controller, self.model, config, getattr(args, 'optimizer', 'adam'))
         self.dis_optimizer, self.dis_lrscheduler = get_dis_optimizer_scheduler(self.discriminator, config)
         self.model_criterion = task_loss(config)
         self.controller_criterion = search_loss(config)

@@ -3,6 +3,7 @@
 
 Extra, optional flags (not in the reference): --crop_size (the reference hard-codes 256),
 --backbone_dtype {f32x3,fp32,bf16} (default f32x3: the own float32-precision convolution kernels), --max_epochs / --epoch_items (short synthetic runs), --sync_bn / --placement (multi-GPU),
+--optimizer {adam,muon},
 --fixed_policy."""
 import argparse
 import sys
@@ -38,6 +39,9 @@ def parse_args(argv=None):
                              "contract, tests/test_gpu_precision.py) -- layers / backbones they do not cover take the library's float32 convolution "
                              "and are listed on stderr after the first step; fp32: the library's float32 convolutions everywhere (2.2x slower on "
                              "ResNet-50); bf16: bfloat16 autocast (narrower than the reference)")
+    parser.add_argument('--optimizer', default='adam', choices=['adam', 'muon'],
+                        help='optimiser of the segmentation model: adam (the reference) or muon: orthogonalised momentum updates of the weight matrices '
+                             '(aadg_amd/muon.py), Adam for the other parameters, one learning rate for both')
     parser.add_argument('--sync_bn', action='store_true', help='SyncBatchNorm over the row-sharded ranks')
     parser.add_argument('--placement', default='row', choices=['unit', 'row'],
                         help='multi-GPU cut of the domain-major (domain, policy) unit sequence: balanced to the row (default, as bench.py: 18 rows per rank at 8 GPUs) or whole units per rank (SURVEY 8e as written: 3/3/2/... units = 24 rows on the slowest rank); one domain per GPU at 3 GPUs either way')
