@@ -22,6 +22,10 @@ HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-cont
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                "-Wall", "-Wno-unused-function", "-I" + INCLUDE, "-I" + CSRC]
 
+# accumulators in ordinary registers: where vector code touches every product (the softmax, its gradient) the default, accumulation registers,
+# costs a move per value and direction
+SOURCE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def _hipcc():
     exe = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
@@ -55,7 +59,7 @@ def build_hip(force=False, verbose=False):
     for src in sources():
         obj = os.path.join(objdir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
-        cmd = [hipcc] + HIPCC_FLAGS + ["-c", src, "-o", obj]
+        cmd = [hipcc] + HIPCC_FLAGS + SOURCE_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
         if verbose:
             print(" ".join(cmd))
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))

@@ -35,6 +35,7 @@ typedef short at_v4i16 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }     // v_exp_f32: 1 ulp, results below 2^-126 are 0
 
+constexpr float AT_LAZY = 8.0f;                       // base-2 logarithm
 constexpr float AT_LOG2E = 1.4426950408889634f;
 
 struct AtStride { long long b, h, n; };               // elements: batch, head, row (the head dimension itself is contiguous)
@@ -62,6 +63,15 @@ template <> struct At<uint16_t> {
                             aadg_f2bf_pk(c[8 * g + 4], c[8 * g + 5]), aadg_f2bf_pk(c[8 * g + 6], c[8 * g + 7])};
         return __builtin_bit_cast(Frag, p);
     }
+    static __device__ __forceinline__ float dot(Frag a, Frag b, float s) {
+        const at_u32x4 x = __builtin_bit_cast(at_u32x4, a), y = __builtin_bit_cast(at_u32x4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), s);
+            s = fmaf(__uint_as_float(x[i] & 0xFFFF0000u), __uint_as_float(y[i] & 0xFFFF0000u), s);
+        }
+        return s;
+    }
     static __device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
         *reinterpret_cast<uint2*>(p) = make_uint2(aadg_f2bf_pk(a, b), aadg_f2bf_pk(c, d));
     }
@@ -75,6 +85,11 @@ template <> struct At<float> {
         return c;
     }
     static __device__ __forceinline__ Frag pack(const f32x16& c, int g) { return Frag{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]}; }
+    static __device__ __forceinline__ float dot(Frag a, Frag b, float s) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = fmaf(a[i], b[i], s);
+        return s;
+    }
     static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
         *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
     }
@@ -152,19 +167,22 @@ __device__ __forceinline__ int at_limit_max(const AtArgs& a, int L, int row0, in
     return at_limit(a, L, last);
 }
 
+// waves per SIMD the registers are budgeted for: two (256 registers), one for head widths over 64
+template <typename T, int D> constexpr int at_min_waves() { return D == 128 ? 1 : 2; }
+
 // keys per LDS tile: 64; 32 where the next tile's prefetch registers (2 BK D / threads values) would not fit beside the accumulators
 template <typename T, int D, int NW> constexpr int at_bk() { return NW == 1 || (sizeof(T) == 4 && D == 128) ? 32 : 64; }
 
 // ------------------------------------------------------------------------------------------------ forward
 // Workgroup: NW waves of 32 folded rows; keys in tiles of BK through LDS, the next tile's loads in registers during the products.
 template <typename T, int D, int NW, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AtArgs a) {
+__global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_fwd(const AtArgs a) {
     typedef At<T> M;
     typedef Tile<T, D> L_;
     constexpr int BK = at_bk<T, D, NW>(), KS = M::KS, CH = M::CH, U = D / KS, CPR = D / CH, NT = 64 * NW, LD = BK * CPR / NT, DT = D / 32, PG = 16 / (KS / 2), KT = BK / 32;
     __shared__ __attribute__((aligned(16))) T Ks[BK * L_::PITCH];
     __shared__ __attribute__((aligned(16))) T Vs[BK * L_::PITCH];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int sp = SPLIT ? blockIdx.x % a.splits : 0;
     const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
     const int bg = w / a.tiles, tile = a.tiles - 1 - (w - bg * a.tiles), b = bg / a.G, g = bg - b * a.G;      // causal: longest rows first
@@ -178,6 +196,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AtArgs a) {
     int wave_full = limit;                                                    // keys every row of the wave sees
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) wave_full = min(wave_full, __shfl_xor(wave_full, o, 64));
+    wave_full = __builtin_amdgcn_readfirstlane(wave_full);
 
     const T* kb = (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
     const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
@@ -231,14 +250,24 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AtArgs a) {
                 for (int i = 0; i < 16; ++i)
                     s[t][i] = k0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) < limit ? s[t][i] : -INFINITY;
         }
-        float mx = m;
+        // the reference value m of the exponentials follows the maximum only when that has grown by more than AT_LAZY: accumulator and sum
+        // are rescaled in a few tiles instead of every one, p stays below 2^AT_LAZY
+        float mx = s[0][0];
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mc = mx == -INFINITY ? 0.0f : mx * c;
-        const float alpha = at_exp2(fmaf(m, c, -mc));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+        if (__any(mx > m + AT_LAZY)) {
+            const float mn = fmaxf(m, mx), alpha = mn == -INFINITY ? 1.0f : at_exp2(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m;
         float sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < KT; ++t)
@@ -247,12 +276,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AtArgs a) {
                 s[t][i] = at_exp2(fmaf(s[t][i], c, -mc));
                 sum += s[t][i];
             }
-        l = fmaf(l, alpha, sum);
-        m = mx;
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+        l += sum;
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -268,7 +292,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AtArgs a) {
     if (SPLIT) {
         const long long rows = (long long)a.B * a.G * a.R;
         if (h == 0) {
-            a.ml[2 * (sp * rows + flat)] = m * c;
+            a.ml[2 * (sp * rows + flat)] = m;
             a.ml[2 * (sp * rows + flat) + 1] = l;
         }
         float* op = a.part + (sp * rows + flat) * a.d;
@@ -290,7 +314,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AtArgs a) {
             const int col = 32 * t + 8 * i + 4 * h;
             if (col < a.d) M::store4(op + col, acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv, acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv);
         }
-    if (h == 0 && a.lse != nullptr) a.lse[flat] = l == 0.0f ? INFINITY : fmaf(m, c, log2f(l));
+    if (h == 0 && a.lse != nullptr) a.lse[flat] = l == 0.0f ? INFINITY : m + log2f(l);
 }
 
 // joins the splits of the forward: one lane per 4 values of a row
@@ -322,7 +346,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AtArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// D_i = do_i . o_i, one 16-lane group per row
+// D_i = do_i . o_i, one 16-lane group per row (only where dq, whose kernel computes it on the way, is not asked for)
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
     const long long rows = (long long)a.B * a.G * a.R, flat = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -332,19 +356,9 @@ __global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
     const T* op = (const T*)a.o + at_row(a, a.so, b, g, row);
     const T* gp = (const T*)a.dout + at_row(a, a.sdo, b, g, row);
     float s = 0.0f;
-    for (int c = threadIdx.x & 15; c * At<T>::CH < a.d; c += 16) {
-        const uint4 x = *reinterpret_cast<const uint4*>(op + c * At<T>::CH), y = *reinterpret_cast<const uint4*>(gp + c * At<T>::CH);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (At<T>::CH == 4) {
-                s = fmaf(__uint_as_float(xs[i]), __uint_as_float(ys[i]), s);
-            } else {
-                s = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), s);
-                s = fmaf(__uint_as_float(xs[i] & 0xFFFF0000u), __uint_as_float(ys[i] & 0xFFFF0000u), s);
-            }
-        }
-    }
+    typedef typename At<T>::Frag F;
+    for (int c = threadIdx.x & 15; c * At<T>::CH < a.d; c += 16)
+        s = At<T>::dot(*reinterpret_cast<const F*>(op + c * At<T>::CH), *reinterpret_cast<const F*>(gp + c * At<T>::CH), s);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 15) == 0) a.delta[flat] = s;
@@ -352,13 +366,13 @@ __global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
 
 // dq: the forward's walk over the keys with p recomputed; dq^T += K^T ds^T
 template <typename T, int D, int NW, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void k_attn_dq(const AtArgs a) {
+__global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(const AtArgs a) {
     typedef At<T> M;
     typedef Tile<T, D> L_;
     constexpr int BK = at_bk<T, D, NW>(), KS = M::KS, CH = M::CH, U = D / KS, CPR = D / CH, NT = 64 * NW, LD = BK * CPR / NT, DT = D / 32, PG = 16 / (KS / 2), KT = BK / 32;
     __shared__ __attribute__((aligned(16))) T Ks[BK * L_::PITCH];
     __shared__ __attribute__((aligned(16))) T Vs[BK * L_::PITCH];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int sp = SPLIT ? blockIdx.x % a.splits : 0;
     const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
     const int bg = w / a.tiles, tile = a.tiles - 1 - (w - bg * a.tiles), b = bg / a.G, g = bg - b * a.G;
@@ -372,6 +386,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AtArgs a) {
     int wave_full = limit;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) wave_full = min(wave_full, __shfl_xor(wave_full, o, 64));
+    wave_full = __builtin_amdgcn_readfirstlane(wave_full);
     const T* kb = (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
     const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
     const long long flat = ((long long)b * a.G + g) * a.R + row;
@@ -385,7 +400,16 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AtArgs a) {
             gf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(gp, 0, live ? 0 : 1, 1, 2 * u + h, a.d));
         }
     }
-    const float lse = live ? a.lse[flat] : INFINITY, dl = live ? a.delta[flat] : 0.0f;
+    const float lse = live ? a.lse[flat] : INFINITY;
+    float dl = 0.0f;                                                          // D_i, left for the dk / dv kernel
+    {
+        const T* yp = (const T*)a.o + at_row(a, a.so, b, g, live ? row : 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            dl = M::dot(__builtin_bit_cast(typename M::Frag, at_load<T>(yp, 0, live ? 0 : 1, 1, 2 * u + h, a.d)), gf[u], dl);
+        dl += __shfl_xor(dl, 32, 64);
+        if (live && h == 0 && sp == 0) a.delta[flat] = dl;
+    }
     const float c = a.scale * AT_LOG2E;
     f32x16 acc[DT];
 #pragma unroll
@@ -418,14 +442,17 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AtArgs a) {
         for (int t = 0; t < KT; ++t) {
             f32x16 s, dp;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+            for (int i = 0; i < 16; ++i) {
+                s[i] = 0.0f;
+                dp[i] = -dl;
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 s = M::mma(L_::rows(Ks, 32 * t, u, lane), qf[u], s);
                 dp = M::mma(L_::rows(Vs, 32 * t, u, lane), gf[u], dp);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = at_exp2(fmaf(s[i], c, -lse)) * (dp[i] - dl);
+            for (int i = 0; i < 16; ++i) s[i] = at_exp2(fmaf(s[i], c, -lse)) * dp[i];
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = k0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) < limit ? s[i] : 0.0f;
@@ -454,30 +481,30 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AtArgs a) {
         }
 }
 
-// dk, dv: a wave owns 32 keys (its K and V fragments stay in registers) and walks the folded rows in tiles of 32;
-// dv^T += dO^T P, dk^T += Q^T dS
+// dk, dv: a wave owns 32 keys (its K and V fragments stay in registers) and walks the folded rows, BQ at a time through LDS;
+// dv^T += dO^T P, dk^T += Q^T dS.  -D_i is the initial value of the dP accumulators.
 template <typename T, int D, int NW, bool SPLIT>
-__global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AtArgs a) {
+__global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(const AtArgs a) {
     typedef At<T> M;
     typedef Tile<T, D> L_;
-    constexpr int BQ = 32, KS = M::KS, CH = M::CH, U = D / KS, CPR = D / CH, NT = 64 * NW, LD = (BQ * CPR + NT - 1) / NT, DT = D / 32, PG = 16 / (KS / 2);
+    constexpr int BQ = NW == 1 || D == 128 || sizeof(T) == 4 ? 32 : 64, KS = M::KS, CH = M::CH, U = D / KS, CPR = D / CH, NT = 64 * NW;
+    constexpr int LD = (BQ * CPR + NT - 1) / NT, DT = D / 32, PG = 16 / (KS / 2);
     __shared__ __attribute__((aligned(16))) T Qs[BQ * L_::PITCH];
     __shared__ __attribute__((aligned(16))) T Gs[BQ * L_::PITCH];
     __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
-    __shared__ int Es[BQ];                                                   // key limit of each row
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
+    __shared__ __attribute__((aligned(16))) int Es[BQ];                       // key limit of each row
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int sp = SPLIT ? blockIdx.x % a.splits : 0;
     const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
     const int bg = w / a.tiles, tile = w - bg * a.tiles, b = bg / a.G, g = bg - b * a.G;
     const int L = at_len(a, b);
-    const int key0 = tile * 32 * NW + 32 * wv, key = key0 + (lane & 31);
+    const int wg_key0 = tile * 32 * NW, key0 = wg_key0 + 32 * wv, key = key0 + (lane & 31);
     const T* kb = (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
     const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
     const float c = a.scale * AT_LOG2E;
-    const int r_lo = SPLIT ? sp * a.chunk : 0, r_hi = SPLIT ? min(a.R, r_lo + a.chunk) : a.R;
-    const bool any = tile * 32 * NW < L;                                      // (workgroup-uniform)
+    const int r_lo = SPLIT ? sp * a.chunk : 0, r_hi = wg_key0 < L ? (SPLIT ? min(a.R, r_lo + a.chunk) : a.R) : r_lo;      // (no key: nothing to walk)
     typename M::Frag kf[U], vf[U];
-    if (any) {
+    if (wg_key0 < L) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             kf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(kb, a.sk.n, key, L, 2 * u + h, a.d));
@@ -489,55 +516,102 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AtArgs a) {
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) ak[t][i] = av[t][i] = 0.0f;
-    if (any) {
-        for (int q0 = r_lo; q0 < r_hi; q0 += BQ) {
-            if (a.causal && at_limit_max(a, L, q0, BQ) <= tile * 32 * NW) continue;      // (workgroup-uniform) no row of the tile sees a key of this workgroup
-            __syncthreads();
+    // first tile from q0 on with a row that sees a key of this workgroup
+    auto next = [&](int q0) {
+        if (a.causal)
+            while (q0 < r_hi && at_limit_max(a, L, q0, BQ) <= wg_key0) q0 += BQ;
+        return q0;
+    };
+    uint4 rq[LD], rg[LD];
+    float r_lse = 0.0f, r_d = 0.0f;
+    int r_lim = 0;
+    auto fetch = [&](int q0) {
 #pragma unroll
-            for (int i = 0; i < LD; ++i) {
-                const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
-                if (id >= BQ * CPR) break;
-                const int rr = q0 + rw;
-                const bool ok = rr < r_hi;
-                const uint4 x = at_load<T>((const T*)a.q + at_row(a, a.sq, b, g, ok ? rr : q0), 0, ok ? 0 : 1, 1, ch, a.d);
-                const uint4 y = at_load<T>((const T*)a.dout + at_row(a, a.sdo, b, g, ok ? rr : q0), 0, ok ? 0 : 1, 1, ch, a.d);
-                *reinterpret_cast<uint4*>(&Qs[L_::at(rw, ch)]) = x;
-                *reinterpret_cast<uint4*>(&Gs[L_::at(rw, ch)]) = y;
-            }
-            if (tid < BQ) {
-                const int rr = q0 + tid;
-                const bool ok = rr < r_hi;
-                const long long f = ((long long)b * a.G + g) * a.R + (ok ? rr : q0);
-                Ls[tid] = ok ? a.lse[f] : INFINITY;
-                Ds[tid] = ok ? a.delta[f] : 0.0f;
-                Es[tid] = ok ? at_limit(a, L, rr) : 0;
-            }
-            __syncthreads();
+        for (int i = 0; i < LD; ++i) {
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR, rr = q0 + rw;
+            const bool ok = rr < r_hi && (BQ * CPR % NT == 0 || id < BQ * CPR);
+            const int rc = ok ? rr : q0;
+            rq[i] = at_load<T>((const T*)a.q + at_row(a, a.sq, b, g, rc), 0, ok ? 0 : 1, 1, ch, a.d);
+            rg[i] = at_load<T>((const T*)a.dout + at_row(a, a.sdo, b, g, rc), 0, ok ? 0 : 1, 1, ch, a.d);
+        }
+        if (tid < BQ) {
+            const int rr = q0 + tid;
+            const bool ok = rr < r_hi;
+            const long long f = ((long long)b * a.G + g) * a.R + (ok ? rr : q0);
+            r_lse = ok ? a.lse[f] : INFINITY;
+            r_d = ok ? -a.delta[f] : 0.0f;
+            r_lim = ok ? at_limit(a, L, rr) : 0;
+        }
+    };
+    int q0 = next(r_lo);
+    if (q0 < r_hi) fetch(q0);
+    while (q0 < r_hi) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
+            if (BQ * CPR % NT != 0 && id >= BQ * CPR) break;
+            *reinterpret_cast<uint4*>(&Qs[L_::at(rw, ch)]) = rq[i];
+            *reinterpret_cast<uint4*>(&Gs[L_::at(rw, ch)]) = rg[i];
+        }
+        if (tid < BQ) {
+            Ls[tid] = r_lse;
+            Ds[tid] = r_d;
+            Es[tid] = r_lim;
+        }
+        __syncthreads();
+        const int qn = next(q0 + BQ);
+        if (qn < r_hi) fetch(qn);
+        // a row that does not exist has lse = inf, i.e. p = 0: only the rows' limits can cut this wave's keys
+        const bool edge = a.causal || key0 + 32 > L;
+#pragma unroll
+        for (int t = 0; t < BQ / 32; ++t) {
             f32x16 s, dp;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const aadg_f32x4 x = *reinterpret_cast<const aadg_f32x4*>(&Ds[32 * t + 8 * i + 4 * h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[4 * i + e] = 0.0f;
+                    dp[4 * i + e] = x[e];
+                }
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                s = M::mma(L_::rows(Qs, 0, u, lane), kf[u], s);
-                dp = M::mma(L_::rows(Gs, 0, u, lane), vf[u], dp);
+                s = M::mma(L_::rows(Qs, 32 * t, u, lane), kf[u], s);
+                dp = M::mma(L_::rows(Gs, 32 * t, u, lane), vf[u], dp);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int rr = 8 * (i >> 2) + 4 * h + (i & 3);
-                const float p = key < Es[rr] ? at_exp2(fmaf(s[i], c, -Ls[rr])) : 0.0f;
-                s[i] = p;
-                dp[i] = key < Es[rr] ? p * (dp[i] - Ds[rr]) : 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const aadg_f32x4 x = *reinterpret_cast<const aadg_f32x4*>(&Ls[32 * t + 8 * i + 4 * h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[4 * i + e] = at_exp2(fmaf(s[4 * i + e], c, -x[e]));
             }
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int4 x = *reinterpret_cast<const int4*>(&Es[32 * t + 8 * i + 4 * h]);
+                    const int lim[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[4 * i + e] = key < lim[e] ? s[4 * i + e] : 0.0f;
+                        dp[4 * i + e] = key < lim[e] ? dp[4 * i + e] : 0.0f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
 #pragma unroll
             for (int p = 0; p < PG; ++p) {
                 const typename M::Frag pf = M::pack(s, p), df = M::pack(dp, p);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    av[dt] = M::mma(L_::cols(Gs, KS * p, 32 * dt, lane), pf, av[dt]);
-                    ak[dt] = M::mma(L_::cols(Qs, KS * p, 32 * dt, lane), df, ak[dt]);
+                    av[dt] = M::mma(L_::cols(Gs, 32 * t + KS * p, 32 * dt, lane), pf, av[dt]);
+                    ak[dt] = M::mma(L_::cols(Qs, 32 * t + KS * p, 32 * dt, lane), df, ak[dt]);
                 }
             }
         }
+        q0 = qn;
     }
     if (key >= a.Nk) return;
     const float sc = a.scale;
@@ -673,8 +747,21 @@ template <typename T> int at_forward(AtArgs& a, const AtPlan& p, hipStream_t st)
 
 template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, hipStream_t st) {
     const long long rows = (long long)a.B * a.H * a.Nq;
-    hipLaunchKernelGGL(k_attn_delta<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
-    AADG_LAUNCH_CHECK();
+    if (a.dq != nullptr) {
+        const AtPlan p = at_plan_rows(s);
+        at_use(a, p);
+        AT_BY_D(k_attn_dq, T);                                                // leaves D_i in a.delta
+        AADG_LAUNCH_CHECK();
+        if (p.splits > 1) {
+            const long long n = rows * (a.d / 4);
+            hipLaunchKernelGGL(k_attn_sum<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a.part, (T*)a.dq, a.sdq, a.B, a.H, a.Nq, a.d,
+                               p.splits, rows * a.d);
+            AADG_LAUNCH_CHECK();
+        }
+    } else {
+        hipLaunchKernelGGL(k_attn_delta<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
+        AADG_LAUNCH_CHECK();
+    }
     if (a.dk != nullptr) {
         const AtPlan p = at_plan_keys(s);
         at_use(a, p);
@@ -686,18 +773,6 @@ template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, h
             hipLaunchKernelGGL(k_attn_sum<T>, grid, dim3(256), 0, st, a.part, (T*)a.dk, a.sdk, a.B, a.G, a.Nk, a.d, p.splits, 2 * nk * a.d);
             AADG_LAUNCH_CHECK();
             hipLaunchKernelGGL(k_attn_sum<T>, grid, dim3(256), 0, st, a.part + nk * a.d, (T*)a.dv, a.sdv, a.B, a.G, a.Nk, a.d, p.splits, 2 * nk * a.d);
-            AADG_LAUNCH_CHECK();
-        }
-    }
-    if (a.dq != nullptr) {
-        const AtPlan p = at_plan_rows(s);
-        at_use(a, p);
-        AT_BY_D(k_attn_dq, T);
-        AADG_LAUNCH_CHECK();
-        if (p.splits > 1) {
-            const long long n = rows * (a.d / 4);
-            hipLaunchKernelGGL(k_attn_sum<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a.part, (T*)a.dq, a.sdq, a.B, a.H, a.Nq, a.d,
-                               p.splits, rows * a.d);
             AADG_LAUNCH_CHECK();
         }
     }
@@ -720,7 +795,7 @@ extern "C" size_t aadg_attention_backward_workspace_bytes(const aadg_attention_d
     const size_t row = (size_t)desc_host->d * 4;
     const size_t nk = pk.splits > 1 ? (size_t)pk.splits * 2 * desc_host->B * desc_host->G * desc_host->Nk * row : 0;
     const size_t nq = pq.splits > 1 ? (size_t)pq.splits * desc_host->B * desc_host->H * desc_host->Nq * row : 0;
-    return at_delta_bytes(desc_host) + (nk > nq ? nk : nq);          // dk / dv are joined before dq reuses the partials
+    return at_delta_bytes(desc_host) + (nk > nq ? nk : nq);          // dq is joined before dk / dv reuse the partials
 }
 
 extern "C" int aadg_attention_forward(const aadg_attention_desc* desc_host, const void* q, const void* k, const void* v, const int* key_lengths,
