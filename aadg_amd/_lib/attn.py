@@ -1,6 +1,7 @@
 """Softmax attention of the transformer blocks (csrc/attention.hip): forward, and the backward that recomputes the probabilities."""
-import ctypes
+import contextlib
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -8,25 +9,20 @@ from torch.autograd.function import once_differentiable
 from .binding import AadgError, _check, _ptr, _stream, load
 
 _ATTN_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
-_I64x3 = ctypes.c_int64 * 3
+_ATTN_DESC = struct.Struct("<8ifi24q")             # aadg_attention_desc (include/aadg_hip.h): 8 sizes, scale, a reserved word, 8 x (batch, head, row) strides
+_NO_STRIDE = (0, 0, 0)
 
 
-class _AttentionDesc(ctypes.Structure):
-    """mirror of aadg_attention_desc (include/aadg_hip.h)"""
-    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "B", "H", "G", "Nq", "Nk", "d", "causal")] +
-                [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)] +
-                [(n + "_stride", _I64x3) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv")])
-
-
-def _strides(t):
-    """(batch, head, row) strides in elements; an axis of length 1 is never stepped over."""
-    return _I64x3(*(st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride()[:3])))
+def _attn_desc(dtype, B, H, G, Nq, Nk, d, causal, scale, *strides):
+    flat = [x for st in strides for x in st[:3]]
+    return _ATTN_DESC.pack(dtype, B, H, G, Nq, Nk, d, causal, scale, 0, *flat, *(0,) * (24 - len(flat)))
 
 
 def _rows16(t):
-    """t itself if the kernels can read it in place (contiguous rows, every row on a 16-byte boundary), else a contiguous copy."""
+    """t itself if the kernels can read it in place (contiguous rows, everything on 16-byte boundaries), else a contiguous copy."""
+    a, b, c, e = t.stride()
     unit = 16 // t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(st % unit == 0 or n <= 1 for n, st in zip(t.shape[:3], t.stride()[:3])):
+    if e == 1 and not (a | b | c) % unit and not t.data_ptr() % 16:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -37,26 +33,21 @@ def _by_token(like):
     return torch.empty((B, n, h, d), dtype=like.dtype, device=like.device).transpose(1, 2)
 
 
-def _desc(q, k, scale, causal):
-    de = _AttentionDesc()
-    de.dtype = _ATTN_DTYPES[q.dtype]
-    de.B, de.H, de.Nq, de.d = q.shape
-    de.G, de.Nk = k.shape[1], k.shape[2]
-    de.causal, de.scale = int(causal), scale
-    return de
+def _on(device):
+    """the device the launches go to: nothing to do where it is the current one"""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _attention_forward(q, k, v, scale, causal, key_lengths, want_lse):
     lib = load()
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     o = _by_token(q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
-    de = _desc(q, k, scale, causal)
-    de.q_stride, de.k_stride, de.v_stride, de.o_stride = _strides(q), _strides(k), _strides(v), _strides(o)
-    p = ctypes.byref(de)
-    nbytes = lib.aadg_attention_forward_workspace_bytes(p)
+    B, H, Nq, d = q.shape
+    lse = torch.empty((B, H, Nq), dtype=torch.float32, device=q.device) if want_lse else None
+    de = _attn_desc(_ATTN_DTYPES[q.dtype], B, H, k.shape[1], Nq, k.shape[2], d, causal, scale, q.stride(), k.stride(), v.stride(), o.stride())
+    nbytes = lib.aadg_attention_forward_workspace_bytes(de)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _check(lib.aadg_attention_forward(p, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths), o.data_ptr(), _ptr(lse), _ptr(ws), nbytes,
+    _check(lib.aadg_attention_forward(de, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths), o.data_ptr(), _ptr(lse), _ptr(ws), nbytes,
                                       _stream()), "aadg_attention_forward")
     return q, k, v, o, lse
 
@@ -68,7 +59,7 @@ class _Attention(torch.autograd.Function):
         ctx.empty = q.numel() == 0 or k.numel() == 0
         if ctx.empty:
             return torch.zeros_like(q)
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             q, k, v, o, lse = _attention_forward(q, k, v, scale, causal, key_lengths, True)
         ctx.save_for_backward(q, k, v, o, lse, key_lengths)
         return o
@@ -76,38 +67,37 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
         if ctx.empty:
             sq, sk = ctx.shapes
             return (do.new_zeros(sq), do.new_zeros(sk), do.new_zeros(sk), None, None, None)
         q, k, v, o, lse, key_lengths = ctx.saved_tensors
         lib = load()
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             do = _rows16(do)
             dq = _by_token(q) if need_q else None
-            dk, dv = (_by_token(k), _by_token(v)) if need_kv else (None, None)
-            de = _desc(q, k, ctx.scale, ctx.causal)
-            for n, t in (("q", q), ("k", k), ("v", v), ("o", o), ("do", do), ("dq", dq), ("dk", dk), ("dv", dv)):
-                if t is not None:
-                    setattr(de, n + "_stride", _strides(t))
-            p = ctypes.byref(de)
-            nbytes = lib.aadg_attention_backward_workspace_bytes(p)
+            dk, dv = (_by_token(k), _by_token(v)) if need_k or need_v else (None, None)
+            B, H, Nq, d = q.shape
+            st = [_NO_STRIDE if t is None else t.stride() for t in (q, k, v, o, do, dq, dk, dv)]
+            de = _attn_desc(_ATTN_DTYPES[q.dtype], B, H, k.shape[1], Nq, k.shape[2], d, ctx.causal, ctx.scale, *st)
+            nbytes = lib.aadg_attention_backward_workspace_bytes(de)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            _check(lib.aadg_attention_backward(p, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths), o.data_ptr(), lse.data_ptr(),
+            _check(lib.aadg_attention_backward(de, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths), o.data_ptr(), lse.data_ptr(),
                                                do.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), ws.data_ptr(), nbytes, _stream()),
                    "aadg_attention_backward")
-        return dq, dk, dv, None, None, None
+        return dq, dk if need_k else None, dv if need_v else None, None, None, None
 
 
 def attention_supported(q, k, v):
     """True where `attention` takes these tensors: GPU, float32 / bfloat16, [B, H, Nq, d] and [B, G, Nk, d] with H % G == 0, d % 8 == 0, d <= 128."""
     if not (q.is_cuda and q.dtype in _ATTN_DTYPES and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
         return False
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         return False
-    if k.shape[1] == 0 or q.shape[1] % k.shape[1] != 0 or q.shape[3] % 8 != 0 or not 0 < q.shape[3] <= 128:
+    (B, H, Nq, d), (Bk, G, Nk, dk) = q.shape, k.shape
+    if B != Bk or d != dk or G == 0 or H % G != 0 or d % 8 != 0 or not 0 < d <= 128:
         return False
-    return q.numel() == 0 or k.numel() == 0 or bool(load().aadg_attention_supported(ctypes.byref(_desc(q, k, 1.0, False))))
+    return B * H * Nq * Nk == 0 or bool(load().aadg_attention_supported(_attn_desc(_ATTN_DTYPES[q.dtype], B, H, G, Nq, Nk, d, 0, 1.0)))
 
 
 def attention(q, k, v, scale=None, causal=False, key_lengths=None):
@@ -119,11 +109,8 @@ def attention(q, k, v, scale=None, causal=False, key_lengths=None):
     gives zeros and takes no part in any gradient.  Inputs are expected finite (a key that only the causal rule hides included).
 
     Returns [B, H, Nq, d] over [B, Nq, H, d] memory: `.transpose(1, 2).reshape(B, Nq, H * d)` is free.  Differentiable once in q, k, v."""
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-        raise AadgError("attention: expected q [B, H, Nq, d] and k, v [B, G, Nk, d]")
-    for t in (q, k, v):
-        if not t.is_cuda:
-            raise AadgError("aadg_amd kernels need GPU tensors (got %s); there is no CPU path" % t.device)
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise AadgError("aadg_amd kernels need GPU tensors (got %s, %s, %s); there is no CPU path" % (q.device, k.device, v.device))
     if not attention_supported(q, k, v):
         raise AadgError("attention: expected float32 / bfloat16 tensors of one type and device, q [B, H, Nq, d], k and v [B, G, Nk, d], H %% G == 0, "
                         "d %% 8 == 0, d <= 128; got %s %s %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
@@ -133,4 +120,7 @@ def attention(q, k, v, scale=None, causal=False, key_lengths=None):
     if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (q.shape[0],) or not key_lengths.is_contiguous() or
                                     key_lengths.device != q.device):
         raise AadgError("attention: key_lengths must be a contiguous int32 vector with one length per sequence (%d) on %s" % (q.shape[0], q.device))
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) and q.numel() > 0 and k.numel() > 0:
+        with _on(q.device):
+            return _attention_forward(q, k, v, scale, bool(causal), key_lengths, False)[3]
     return _Attention.apply(q, k, v, scale, bool(causal), key_lengths)

@@ -317,32 +317,42 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_fwd(co
     if (h == 0 && a.lse != nullptr) a.lse[flat] = l == 0.0f ? INFINITY : m + log2f(l);
 }
 
-// joins the splits of the forward: one lane per 4 values of a row
+// joins the splits of the forward: one wave per row.  The lanes take the splits' (m, l) at once (at most 64 splits), then groups of d / 4 lanes
+// take every 64 / (d / 4)-th split's partial row; a fixed order throughout.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(const AtArgs a) {
-    const int per = a.d / 4;
-    const long long rows = (long long)a.B * a.G * a.R, id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long flat = id / per;
+    const long long rows = (long long)a.B * a.G * a.R, flat = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (flat >= rows) return;
-    const int col = (int)(id - flat * per) * 4;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s)
-        if (a.ml[2 * (s * rows + flat) + 1] != 0.0f) m = fmaxf(m, a.ml[2 * (s * rows + flat)]);
-    float l = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
-    for (int s = 0; s < a.splits; ++s) {
-        const float ls = a.ml[2 * (s * rows + flat) + 1];
-        if (ls == 0.0f) continue;                                             // no key of this split
-        const float w = at_exp2(a.ml[2 * (s * rows + flat)] - m);
-        const float4 x = *reinterpret_cast<const float4*>(a.part + (s * rows + flat) * a.d + col);
-        l = fmaf(ls, w, l);
-        o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+    const int lane = threadIdx.x & 63, per = a.d / 4, groups = 64 / per, grp = lane / per, col = (lane - grp * per) * 4;
+    float ms = -INFINITY, ls = 0.0f;
+    if (lane < a.splits) {
+        const float2 x = *reinterpret_cast<const float2*>(a.ml + 2 * (lane * rows + flat));
+        ls = x.y;
+        if (ls != 0.0f) ms = x.x;                                             // l = 0: no key of this split, its partial row is not read
     }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    const float m = wave_max(ms);
+    const float wgt = ls != 0.0f ? at_exp2(ms - m) : 0.0f;
+    const float l = wave_sum(ls * wgt);
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int s0 = 0; s0 < a.splits; s0 += groups) {
+        const int s = s0 + grp;
+        const float w = __shfl(wgt, s & 63, 64);
+        if (grp < groups && s < a.splits && w != 0.0f) {
+            const float4 x = *reinterpret_cast<const float4*>(a.part + (s * rows + flat) * a.d + col);
+            o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+        }
+    }
+    float4 t = o;
+    for (int k = 1; k < groups; ++k) {
+        const int from = (lane + k * per) & 63;
+        t.x += __shfl(o.x, from, 64); t.y += __shfl(o.y, from, 64); t.z += __shfl(o.z, from, 64); t.w += __shfl(o.w, from, 64);
+    }
+    if (grp != 0) return;
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);           // NaN stays
     const long long bg = flat / a.R;
     const int b = (int)(bg / a.G), g = (int)(bg - (long long)b * a.G), row = (int)(flat - bg * a.R);
-    At<T>::store4((T*)a.out + at_row(a, a.so, b, g, row) + col, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    if (col == 0 && a.lse != nullptr) a.lse[flat] = l == 0.0f ? INFINITY : m + log2f(l);
+    At<T>::store4((T*)a.out + at_row(a, a.so, b, g, row) + col, t.x * inv, t.y * inv, t.z * inv, t.w * inv);
+    if (lane == 0 && a.lse != nullptr) a.lse[flat] = l == 0.0f ? INFINITY : m + log2f(l);
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -638,26 +648,30 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
         }
 }
 
-// sum of the splits' partials in split order, one lane per 4 values: out[b, head, n] = sum_s part[s * step + (b heads + head) n_rows + n]
+// sum of the splits' partials in split order, one lane per 4 values: out[b, head, n] = sum_s part[s * step + (b heads + head) n_rows + n];
+// a second row of workgroups takes a second tensor, whose partials lie behind the first's
 template <typename T>
-__global__ __launch_bounds__(256) void k_attn_sum(const float* __restrict__ part, T* __restrict__ out, AtStride s, int B, int heads, int n_rows,
-                                                  int d, int splits, long long step) {
+__global__ __launch_bounds__(256) void k_attn_sum(const float* __restrict__ part, T* __restrict__ out0, AtStride s0, T* __restrict__ out1, AtStride s1, int B,
+                                                  int heads, int n_rows, int d, int splits, long long step) {
     const int per = d / 4;
     const long long rows = (long long)B * heads * n_rows, id = (long long)blockIdx.x * 256 + threadIdx.x, flat = id / per;
     if (flat >= rows) return;
     const int col = (int)(id - flat * per) * 4;
+    const float* p = part + (blockIdx.y ? rows * d : 0) + flat * d + col;
     float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
     for (int i = 0; i < splits; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(part + i * step + flat * d + col);
+        const float4 x = *reinterpret_cast<const float4*>(p + i * step);
         o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
     }
     const long long bh = flat / n_rows;
     const long long b = bh / heads, hh = bh - b * heads, n = flat - bh * n_rows;
-    At<T>::store4(out + b * s.b + hh * s.h + n * s.n + col, o.x, o.y, o.z, o.w);
+    const AtStride s = blockIdx.y ? s1 : s0;
+    At<T>::store4((blockIdx.y ? out1 : out0) + b * s.b + hh * s.h + n * s.n + col, o.x, o.y, o.z, o.w);
 }
 
 // ------------------------------------------------------------------------------------------------ host
-constexpr int AT_TARGET_WG = 512;                     // two workgroups of 4 waves per CU
+constexpr int AT_TARGET_WAVES = 2048;
 
 AtStride at_stride(const int64_t* s) { return AtStride{s[0], s[1], s[2]}; }
 
@@ -681,16 +695,17 @@ bool at_aligned(const aadg_attention_desc* s, const void* p, const int64_t* st) 
 
 struct AtPlan { int nw, tiles, splits, chunk; };
 
-// waves per workgroup by what there is to own (32 rows a wave); splits of the other axis (in units of `tile`) until the card has
-// AT_TARGET_WG workgroups' worth of waves, each with at least two tiles to amortise the join
+// Waves per workgroup by what there is to own (32 rows a wave).  Splits of the other axis, in units of `tile`, until the card has eight waves per
+// CU; a split keeps at least two tiles if nearly nothing else runs (under a wave per four CUs), eight otherwise: the join is a launch
+// of its own, and what it costs (4 us) eight tiles take.
 AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile) {
     AtPlan p;
     p.nw = own <= 32 ? 1 : 4;
     p.tiles = (own + 32 * p.nw - 1) / (32 * p.nw);
     const int64_t waves = (int64_t)s->B * s->G * p.tiles * p.nw;
-    const int n = (other + tile - 1) / tile;
-    int64_t sp = (4 * AT_TARGET_WG + waves - 1) / waves;
-    if (sp > n / 2) sp = n / 2;
+    const int n = (other + tile - 1) / tile, least = waves < 64 ? 2 : 8;
+    int64_t sp = (AT_TARGET_WAVES + waves - 1) / waves;
+    if (sp > n / least) sp = n / least;
     if (sp > 64) sp = 64;
     if (sp < 1) sp = 1;
     const int per = (int)((n + sp - 1) / sp);
@@ -738,8 +753,8 @@ template <typename T> int at_forward(AtArgs& a, const AtPlan& p, hipStream_t st)
     AT_BY_D(k_attn_fwd, T);
     AADG_LAUNCH_CHECK();
     if (p.splits > 1) {
-        const long long n = (long long)a.B * a.H * a.Nq * (a.d / 4);
-        hipLaunchKernelGGL(k_attn_join<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+        const long long n = (long long)a.B * a.H * a.Nq;
+        hipLaunchKernelGGL(k_attn_join<T>, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, a);
         AADG_LAUNCH_CHECK();
     }
     return 0;
@@ -754,8 +769,8 @@ template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, h
         AADG_LAUNCH_CHECK();
         if (p.splits > 1) {
             const long long n = rows * (a.d / 4);
-            hipLaunchKernelGGL(k_attn_sum<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a.part, (T*)a.dq, a.sdq, a.B, a.H, a.Nq, a.d,
-                               p.splits, rows * a.d);
+            hipLaunchKernelGGL(k_attn_sum<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a.part, (T*)a.dq, a.sdq, (T*)nullptr, a.sdq, a.B,
+                               a.H, a.Nq, a.d, p.splits, rows * a.d);
             AADG_LAUNCH_CHECK();
         }
     } else {
@@ -769,10 +784,8 @@ template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, h
         AADG_LAUNCH_CHECK();
         if (p.splits > 1) {
             const long long nk = (long long)a.B * a.G * a.Nk, n = nk * (a.d / 4);
-            const dim3 grid((unsigned)((n + 255) / 256));
-            hipLaunchKernelGGL(k_attn_sum<T>, grid, dim3(256), 0, st, a.part, (T*)a.dk, a.sdk, a.B, a.G, a.Nk, a.d, p.splits, 2 * nk * a.d);
-            AADG_LAUNCH_CHECK();
-            hipLaunchKernelGGL(k_attn_sum<T>, grid, dim3(256), 0, st, a.part + nk * a.d, (T*)a.dv, a.sdv, a.B, a.G, a.Nk, a.d, p.splits, 2 * nk * a.d);
+            hipLaunchKernelGGL(k_attn_sum<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, st, a.part, (T*)a.dk, a.sdk, (T*)a.dv, a.sdv, a.B,
+                               a.G, a.Nk, a.d, p.splits, 2 * nk * a.d);
             AADG_LAUNCH_CHECK();
         }
     }

@@ -5,14 +5,30 @@ import pytest
 import torch
 
 
+class _Desc(ctypes.Structure):
+    """aadg_attention_desc as include/aadg_hip.h declares it"""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "B", "H", "G", "Nq", "Nk", "d", "causal")] + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)] +
+                [(n + "_stride", ctypes.c_int64 * 3) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv")])
+
+
 def _desc(_lib, **kw):
-    d = _lib._AttentionDesc()
+    d = _Desc()
     for k, v in dict(dtype=1, B=2, H=4, G=2, Nq=8, Nk=16, d=64, causal=0, scale=0.125).items():
         setattr(d, k, kw.pop(k, v))
     for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv"):
         setattr(d, n + "_stride", (ctypes.c_int64 * 3)(*kw.pop(n, (4096, 512, 64))))
     assert not kw
     return d
+
+
+def test_descriptor_layout():
+    from aadg_amd import _lib
+    strides = [(100 * i + 1, 100 * i + 2, 100 * i + 3, 1) for i in range(8)]
+    packed = _lib._attn_desc(1, 2, 4, 2, 8, 16, 64, True, 0.125, *strides)
+    d = _Desc.from_buffer_copy(packed)
+    assert len(packed) == ctypes.sizeof(_Desc)
+    assert (d.dtype, d.B, d.H, d.G, d.Nq, d.Nk, d.d, d.causal, d.scale) == (1, 2, 4, 2, 8, 16, 64, 1, 0.125)
+    assert [list(getattr(d, n + "_stride")) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv")] == [list(s[:3]) for s in strides]
 
 
 def test_attention_entry_points_validate_arguments():
