@@ -696,14 +696,16 @@ bool at_aligned(const aadg_attention_desc* s, const void* p, const int64_t* st) 
 struct AtPlan { int nw, tiles, splits, chunk; };
 
 // Waves per workgroup by what there is to own (32 rows a wave).  Splits of the other axis, in units of `tile`, until the card has eight waves per
-// CU; a split keeps at least two tiles if nearly nothing else runs (under a wave per four CUs), eight otherwise: the join is a launch
-// of its own, and what it costs (4 us) eight tiles take.
+// CU.  The join is a launch of its own (4 us), so a split keeps what takes as long: 256 / D tiles in bfloat16 (1 us a tile at D = 64), two at
+// D = 32 and one otherwise in float32 (5 us at D = 64); two where nearly nothing else runs (under a wave per four CUs) and a tile takes a
+// trip to memory, not its products.
 AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile) {
     AtPlan p;
     p.nw = own <= 32 ? 1 : 4;
     p.tiles = (own + 32 * p.nw - 1) / (32 * p.nw);
     const int64_t waves = (int64_t)s->B * s->G * p.tiles * p.nw;
-    const int n = (other + tile - 1) / tile, least = waves < 64 ? 2 : 8;
+    const int D = s->d <= 32 ? 32 : s->d <= 64 ? 64 : 128, work = s->dtype == 1 ? 256 / D : D == 32 ? 2 : 1;
+    const int n = (other + tile - 1) / tile, least = waves < 64 && work > 2 ? 2 : work;
     int64_t sp = (AT_TARGET_WAVES + waves - 1) / waves;
     if (sp > n / least) sp = n / least;
     if (sp > 64) sp = 64;
