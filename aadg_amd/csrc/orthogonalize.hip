@@ -11,7 +11,7 @@
 // written by the kernel that produces a matrix, once per element; the product kernels move bfloat16 only.
 //
 // All matrices of the list go through each phase in ONE launch: a workgroup finds its matrix from the running tile counts of a table in the
-// workspace.  The table travels in kernel arguments (32 entries a launch), so a captured graph keeps it.
+// workspace.  The table travels in kernel arguments (26 entries a launch), so a captured graph keeps it.
 #include "common.h"
 
 namespace {
@@ -24,15 +24,17 @@ typedef uint32_t or_u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int OR_BK = 32;                             // contracted values per LDS stage
 constexpr int OR_SUM = 16384;                         // elements per workgroup of the norm
-constexpr int OR_CHUNK = 32;                          // table entries per launch (kernel arguments: 4 KB)
+constexpr int OR_CHUNK = 26;                          // table entries per launch (kernel arguments: 4 KB)
 
-enum { OR_P_SUM, OR_P_SPLIT, OR_P_SYM, OR_P_X, OR_PHASES };
+enum { OR_P_SUM, OR_P_SPLIT, OR_P_GRAM, OR_P_SYM, OR_P_X, OR_PHASES };
+enum { OR_B_X0, OR_B_X1, OR_B_A, OR_B_P0, OR_B_P1, OR_B_T, OR_B_Q, OR_BUFS };
 
 struct OrMat {
     const float* src;
     float* dst;
-    long long x0, x1, a, b, sums;                     // byte offsets of the planes and the partial sums in the workspace
+    long long buf[OR_BUFS], sums, part;               // byte offsets of the planes, the norm's and the long products' partial sums in the workspace
     int rows, cols, m, n, ldx, lda;
+    int splits, chunk;                                // pieces of the long axis in A = X X^T
     int first[OR_PHASES];                             // index of the matrix's first workgroup in each phase
     int pad;
 };
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(256) void k_or_planes(const OrMat* __restrict__ tab
     }
     __syncthreads();
     const float scale = scale_s;
-    uint16_t* x = reinterpret_cast<uint16_t*>(ws + t.x0);
+    uint16_t* x = reinterpret_cast<uint16_t*>(ws + t.buf[OR_B_X0]);
     const long long plane = (long long)t.m * t.ldx;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -141,33 +143,125 @@ template <int TB> __device__ __forceinline__ or_bf16x8 or_cols(const uint16_t* t
     return __builtin_bit_cast(or_bf16x8, v);
 }
 
+// 8 values -> one 16-byte store per plane
+__device__ __forceinline__ void or_store8(uint16_t* p, long long plane, const float* v) {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float x = v[2 * i], y = v[2 * i + 1];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            w[k][i] = aadg_f2bf_pk(x, y);
+            x -= __uint_as_float(w[k][i] << 16);
+            y -= __uint_as_float(w[k][i] & 0xFFFF0000u);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(p + k * plane) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+}
+__device__ __forceinline__ void or_load8(const uint16_t* p, long long plane, float* v) {
+    uint4 w[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) w[k] = *reinterpret_cast<const uint4*>(p + k * plane);
+    const uint32_t a[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, b[4] = {w[1].x, w[1].y, w[1].z, w[1].w}, c[4] = {w[2].x, w[2].y, w[2].z, w[2].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(a[i] << 16) + (__uint_as_float(b[i] << 16) + __uint_as_float(c[i] << 16));
+        v[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u) + (__uint_as_float(b[i] & 0xFFFF0000u) + __uint_as_float(c[i] & 0xFFFF0000u));
+    }
+}
+
+// what one product of a phase does: out = ca L R + cb E + cd I over the buffers of OrMat::buf (e < 0: no E).  Two of them: blockIdx.y.
+struct OrOp { int l, r, o, e; float ca, cb, cd; };
+struct OrOps { OrOp op[2]; };
+
+// tile index -> (ti, tj), tj <= ti: w = ti (ti + 1) / 2 + tj
+__device__ __forceinline__ void or_triangle(int w, int& ti, int& tj) {
+    ti = (int)((sqrtf(8.0f * w + 1.0f) - 1.0f) * 0.5f);
+    while (ti * (ti + 1) / 2 > w) --ti;
+    while ((ti + 1) * (ti + 2) / 2 <= w) ++ti;
+    tj = w - ti * (ti + 1) / 2;
+}
+
+// the finished tile, in LDS as float32 [TB][TB + 8], to the planes of a symmetric matrix: at (ti, tj), and mirrored at (tj, ti)
+template <int TB>
+__device__ __forceinline__ void or_store_symmetric(const OrMat& t, const float* tile, int ti, int tj, const OrOp& op, char* ws) {
+    constexpr int TP = TB + 8, C8 = TB / 8;
+    const int m = t.m, lda = t.lda;
+    const long long plane = (long long)m * lda;
+    uint16_t* out = reinterpret_cast<uint16_t*>(ws + t.buf[op.o]);
+    const uint16_t* E = op.e < 0 ? nullptr : reinterpret_cast<const uint16_t*>(ws + t.buf[op.e]);
+    const int i0 = ti * TB, j0 = tj * TB;
+#pragma unroll 2
+    for (int id = threadIdx.x; id < TB * C8; id += 256) {
+        const int r = id / C8, c = (id - r * C8) * 8, row = i0 + r, col = j0 + c;
+        if (row >= m || col >= lda) continue;
+        float v[8], e[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = tile[r * TP + c + x] * op.ca;
+        if (E != nullptr) {
+            or_load8(E + (long long)row * lda + col, plane, e);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = fmaf(op.cb, e[x], v[x]);
+        }
+        if (op.cd != 0.0f) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] += row == col + x ? op.cd : 0.0f;
+        }
+        or_store8(out + (long long)row * lda + col, plane, v);
+    }
+    if (ti == tj) return;
+#pragma unroll 2
+    for (int id = threadIdx.x; id < TB * C8; id += 256) {                    // mirrored row = the tile's column: neighbouring lanes, neighbouring columns
+        const int r8 = id / TB * 8, c = id - id / TB * TB, row = j0 + c, col = i0 + r8;
+        if (row >= m || col >= lda) continue;
+        float v[8], e[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = tile[(r8 + x) * TP + c] * op.ca;
+        if (E != nullptr) {
+            or_load8(E + (long long)row * lda + col, plane, e);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = fmaf(op.cb, e[x], v[x]);
+        }
+        or_store8(out + (long long)row * lda + col, plane, v);
+    }
+}
+
 // One TB x TB tile of a product, 4 waves of (TB / 2) x (TB / 2).
-//   PH = OR_A: A = X X^T          (tiles i >= j, stored twice)
-//   PH = OR_B: B = b A + c A A    (A symmetric: A A^T; tiles i >= j, stored twice)
-//   PH = OR_X: X' = a X + B X     (the second operand K-strided: transpose reads); last step: to the caller's matrix instead
-enum { OR_A, OR_B, OR_X };
+//   PH = OR_GRAM: L = R = X (K = n, cut into t.splits pieces; more than one: the partial tile goes to the workspace for k_or_reduce), symmetric
+//   PH = OR_SYM:  L, R symmetric matrices that commute, the product symmetric
+//   PH = OR_X:    L symmetric, R = X, the K-strided operand (transpose reads); `last`: the result goes to the caller's matrix
+// Of a symmetric product the tiles tj <= ti are computed and stored twice.
+enum { OR_GRAM, OR_SYM, OR_X };
 template <int PH, int TB>
-__global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table, int count, char* __restrict__ ws, float ca, float cb, int odd, int last) {
+__global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table, int count, char* __restrict__ ws, const OrOps ops, int last) {
     constexpr int W = TB / 64, LR = 3 * TB * (OR_BK / 8) / 256;             // 32-wide blocks per wave side; 16-byte chunks per thread and operand
-    __shared__ __attribute__((aligned(16))) uint16_t Ls[3 * TB * OR_BK], Rs[3 * TB * OR_BK];
-    const OrMat t = table[or_find(table, count, PH == OR_X ? OR_P_X : OR_P_SYM, blockIdx.x)];
+    constexpr int TP = TB + 8, STAGE = 2 * 3 * TB * OR_BK * 2, BYTES = STAGE > TB * TP * 4 ? STAGE : TB * TP * 4;
+    __shared__ __attribute__((aligned(16))) char lds[BYTES];
+    uint16_t *Ls = reinterpret_cast<uint16_t*>(lds), *Rs = Ls + 3 * TB * OR_BK;
+    constexpr int PHASE = PH == OR_GRAM ? OR_P_GRAM : PH == OR_SYM ? OR_P_SYM : OR_P_X;
+    const OrMat& t = table[or_find(table, count, PHASE, blockIdx.x)];
+    const OrOp op = ops.op[blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
-    int w = blockIdx.x - t.first[PH == OR_X ? OR_P_X : OR_P_SYM], ti, tj;
+    int w = blockIdx.x - t.first[PHASE], ti, tj, k_lo = 0, sp = 0;
+    const uint16_t* L = reinterpret_cast<const uint16_t*>(ws + t.buf[op.l]);
+    const uint16_t* R = reinterpret_cast<const uint16_t*>(ws + t.buf[op.r]);
+    const int m = t.m, ldl = PH == OR_GRAM ? t.ldx : t.lda, ldr = PH == OR_SYM ? t.lda : t.ldx;
+    int K = ldl;
     if (PH == OR_X) {
         const int tn = (t.ldx + TB - 1) / TB;
         ti = w / tn;
         tj = w - ti * tn;
-    } else {                                                               // w = ti (ti + 1) / 2 + tj, tj <= ti
-        ti = (int)((sqrtf(8.0f * w + 1.0f) - 1.0f) * 0.5f);
-        while (ti * (ti + 1) / 2 > w) --ti;
-        while ((ti + 1) * (ti + 2) / 2 <= w) ++ti;
-        tj = w - ti * (ti + 1) / 2;
+    } else {
+        if (PH == OR_GRAM) {
+            sp = w % t.splits;
+            w /= t.splits;
+            k_lo = sp * t.chunk;
+            K = min(K, k_lo + t.chunk);
+        }
+        or_triangle(w, ti, tj);
     }
-    const uint16_t* X = reinterpret_cast<const uint16_t*>(ws + (odd ? t.x1 : t.x0));
-    const uint16_t* L = PH == OR_A ? X : reinterpret_cast<const uint16_t*>(ws + (PH == OR_B ? t.a : t.b));
-    const uint16_t* R = PH == OR_B ? L : X;
-    const int ldl = PH == OR_A ? t.ldx : t.lda, ldr = PH == OR_B ? t.lda : t.ldx, K = PH == OR_A ? t.ldx : t.lda;
-    const long long pl_l = (long long)t.m * ldl, pl_r = (long long)t.m * ldr;
+    const long long pl_l = (long long)m * ldl, pl_r = (long long)m * ldr;
     const int i0 = ti * TB, j0 = tj * TB, wi = (wv >> 1) * (TB / 2), wj = (wv & 1) * (TB / 2);
 
     uint4 rl[LR], rr[LR];
@@ -177,17 +271,17 @@ __global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table,
             const int id = tid + 256 * i;
             {
                 const int pl = id / (TB * 4), q = id - pl * (TB * 4), row = i0 + (q >> 2), k = k0 + (q & 3) * 8;
-                const uint4 x = *reinterpret_cast<const uint4*>(L + pl * pl_l + (long long)min(row, t.m - 1) * ldl + min(k, ldl - 8));
-                rl[i] = row < t.m && k < ldl ? x : make_uint4(0, 0, 0, 0);
+                const uint4 x = *reinterpret_cast<const uint4*>(L + pl * pl_l + (long long)min(row, m - 1) * ldl + min(k, ldl - 8));
+                rl[i] = row < m && k < ldl ? x : make_uint4(0, 0, 0, 0);
             }
             if (PH != OR_X) {
                 const int pl = id / (TB * 4), q = id - pl * (TB * 4), row = j0 + (q >> 2), k = k0 + (q & 3) * 8;
-                const uint4 x = *reinterpret_cast<const uint4*>(R + pl * pl_r + (long long)min(row, t.m - 1) * ldr + min(k, ldr - 8));
-                rr[i] = row < t.m && k < ldr ? x : make_uint4(0, 0, 0, 0);
+                const uint4 x = *reinterpret_cast<const uint4*>(R + pl * pl_r + (long long)min(row, m - 1) * ldr + min(k, ldr - 8));
+                rr[i] = row < m && k < ldr ? x : make_uint4(0, 0, 0, 0);
             } else {
                 const int pl = id / (OR_BK * (TB / 8)), q = id - pl * (OR_BK * (TB / 8)), k = k0 + q / (TB / 8), c = j0 + (q % (TB / 8)) * 8;
-                const uint4 x = *reinterpret_cast<const uint4*>(R + pl * pl_r + (long long)min(k, t.m - 1) * ldr + min(c, ldr - 8));
-                rr[i] = k < t.m && c < ldr ? x : make_uint4(0, 0, 0, 0);
+                const uint4 x = *reinterpret_cast<const uint4*>(R + pl * pl_r + (long long)min(k, m - 1) * ldr + min(c, ldr - 8));
+                rr[i] = k < m && c < ldr ? x : make_uint4(0, 0, 0, 0);
             }
         }
     };
@@ -198,8 +292,8 @@ __global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table,
         for (int y = 0; y < W; ++y)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[x][y][i] = 0.0f;
-    fetch(0);
-    for (int k0 = 0; k0 < K; k0 += OR_BK) {
+    fetch(k_lo);
+    for (int k0 = k_lo; k0 < K; k0 += OR_BK) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < LR; ++i) {
@@ -248,55 +342,77 @@ __global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table,
                 }
         }
     }
-    // epilogue: register i of half h = row 8 (i / 4) + 4 h + i % 4, lane & 31 = column
-    uint16_t* out = reinterpret_cast<uint16_t*>(ws + (PH == OR_A ? t.a : PH == OR_B ? t.b : odd ? t.x0 : t.x1));
-    const int ldo = PH == OR_X ? t.ldx : t.lda;
-    const long long pl_o = (long long)t.m * ldo;
-    const bool tall = t.rows > t.cols;
+    // the tile goes through LDS (register i of half h = row 8 (i / 4) + 4 h + i % 4, lane & 31 = column: 2-byte stores of the planes straight from
+    // the registers took longer than the product): pitch TB + 8 words, the two halves of a write 32 banks apart
+    float* tile = reinterpret_cast<float*>(lds);
+    __syncthreads();
 #pragma unroll
     for (int x = 0; x < W; ++x)
 #pragma unroll
-        for (int y = 0; y < W; ++y) {
-            const int col = j0 + wj + 32 * y + (lane & 31);
+        for (int y = 0; y < W; ++y)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int row = i0 + wi + 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
-                float v = acc[x][y][i];
-                if (PH == OR_X) {
-                    if (row >= t.m || col >= t.ldx) continue;
-                    const long long e = (long long)row * ldo + col;
-                    v = fmaf(ca, or_join(X[e], X[pl_o + e], X[2 * pl_o + e]), v);
-                    if (last) {
-                        if (col < t.n) t.dst[tall ? (long long)col * t.cols + row : (long long)row * t.cols + col] = v;
-                        continue;
-                    }
-                    uint16_t p[3];
-                    or_split(v, p);
-#pragma unroll
-                    for (int k = 0; k < 3; ++k) out[k * pl_o + e] = p[k];
-                } else {
-                    const long long e = (long long)row * ldo + col, f = (long long)col * ldo + row;
-                    const bool in = row < t.m && col < t.lda, mirror = ti != tj && col < t.m && row < t.lda;
-                    if (PH == OR_B) {
-                        const bool have = row < t.m && col < t.m;
-                        v = have ? fmaf(cb, v, ca * or_join(L[e], L[pl_o + e], L[2 * pl_o + e])) : 0.0f;
-                    }
-                    uint16_t p[3];
-                    or_split(v, p);
-#pragma unroll
-                    for (int k = 0; k < 3; ++k) {
-                        if (in) out[k * pl_o + e] = p[k];
-                        if (mirror) out[k * pl_o + f] = p[k];
-                    }
-                }
-            }
+            for (int i = 0; i < 16; ++i) tile[(wi + 32 * x + 8 * (i >> 2) + 4 * h + (i & 3)) * TP + wj + 32 * y + (lane & 31)] = acc[x][y][i];
+    __syncthreads();
+    if (PH == OR_GRAM && t.splits > 1) {
+        float4* part = reinterpret_cast<float4*>(ws + t.part) + ((long long)w * t.splits + sp) * (TB * TB / 4);
+        for (int id = tid; id < TB * TB / 4; id += 256) {
+            const int r = id / (TB / 4), c = (id - r * (TB / 4)) * 4;
+            part[id] = *reinterpret_cast<const float4*>(&tile[r * TP + c]);
         }
+        return;
+    }
+    if (PH != OR_X) {
+        or_store_symmetric<TB>(t, tile, ti, tj, op, ws);
+        return;
+    }
+    if (!last) {
+        uint16_t* out = reinterpret_cast<uint16_t*>(ws + t.buf[op.o]);
+        for (int id = tid; id < TB * (TB / 8); id += 256) {
+            const int r = id / (TB / 8), c = (id - r * (TB / 8)) * 8;
+            if (i0 + r >= t.m || j0 + c >= t.ldx) continue;
+            float v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = tile[r * TP + c + x];
+            or_store8(out + (long long)(i0 + r) * t.ldx + j0 + c, pl_r, v);
+        }
+        return;
+    }
+    const bool tall = t.rows > t.cols;
+    for (int id = tid; id < TB * TB; id += 256) {                             // lanes along the rows of the caller's matrix
+        const int x = id / TB, y = id - x * TB, r = tall ? y : x, c = tall ? x : y;
+        if (i0 + r < t.m && j0 + c < t.n) t.dst[tall ? (long long)(j0 + c) * t.cols + i0 + r : (long long)(i0 + r) * t.cols + j0 + c] = tile[r * TP + c];
+    }
+}
+
+// joins the pieces of the long products A = X X^T in order
+template <int TB>
+__global__ __launch_bounds__(256) void k_or_reduce(const OrMat* __restrict__ table, int count, char* __restrict__ ws, const OrOps ops) {
+    constexpr int TP = TB + 8;
+    __shared__ __attribute__((aligned(16))) float tile[TB * TP];
+    const OrMat& t = table[or_find(table, count, OR_P_SYM, blockIdx.x)];
+    if (t.splits == 1) return;                                                // (stored by the product itself)
+    const int w = blockIdx.x - t.first[OR_P_SYM];
+    int ti, tj;
+    or_triangle(w, ti, tj);
+    const float4* part = reinterpret_cast<const float4*>(ws + t.part) + (long long)w * t.splits * (TB * TB / 4);
+    for (int id = threadIdx.x; id < TB * TB / 4; id += 256) {
+        float4 s = part[id];
+#pragma unroll 4
+        for (int k = 1; k < t.splits; ++k) {
+            const float4 x = part[(long long)k * (TB * TB / 4) + id];
+            s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        }
+        const int r = id / (TB / 4), c = (id - r * (TB / 4)) * 4;
+        *reinterpret_cast<float4*>(&tile[r * TP + c]) = s;
+    }
+    __syncthreads();
+    or_store_symmetric<TB>(t, tile, ti, tj, ops.op[0], ws);
 }
 
 // ------------------------------------------------------------------------------------------------ host
 constexpr int OR_MAX_SIDE = 1 << 16, OR_MAX_MATS = 4096;
 
-struct OrLayout { size_t bytes; long long grid[OR_PHASES]; int tb; };
+struct OrLayout { size_t bytes; long long grid[OR_PHASES]; int tb_sym, tb_x; bool split; };
 
 // 0 or an error; fills the entries if `out` is given (n entries)
 int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out) {
@@ -305,14 +421,25 @@ int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out) {
         if (mats[i].rows < 1 || mats[i].cols < 1) return AADG_E_BADARG;
         if (mats[i].rows > OR_MAX_SIDE || mats[i].cols > OR_MAX_SIDE || (long long)mats[i].rows * mats[i].cols > (1 << 28)) return AADG_E_UNSUPPORTED;
     }
-    long long big = 0;
+    // tiles of 128 (twice the products per LDS byte of 64) where a phase then still has a workgroup for every CU
+    long long sym = 0, rect = 0;
     for (int i = 0; i < n; ++i) {
         const long long m = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, k = (m + 127) / 128;
-        big += k * (k + 1) / 2;
+        sym += k * (k + 1) / 2;
+        rect += k * (((long long)mats[i].rows + mats[i].cols - m + 127) / 128);
     }
-    lay.tb = big >= 256 ? 128 : 64;                   // fewer 128-wide tiles in the smallest phase than CUs: 64
+    lay.tb_sym = sym >= 256 ? 128 : 64;
+    lay.tb_x = rect >= 256 ? 128 : 64;
+    sym = 0;
+    for (int i = 0; i < n; ++i) {
+        const long long m = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, k = (m + lay.tb_sym - 1) / lay.tb_sym;
+        sym += k * (k + 1) / 2;
+    }
+    // pieces of the long axis: about two workgroups per CU, at least 512 values each (16 stages, as long as the join takes)
+    const long long pieces = sym >= 512 ? 1 : (512 + sym - 1) / sym;
     size_t at = aadg_align_up((size_t)n * sizeof(OrMat), 256);
     for (int p = 0; p < OR_PHASES; ++p) lay.grid[p] = 0;
+    lay.split = false;
     for (int i = 0; i < n; ++i) {
         OrMat t = {};
         t.src = mats[i].src; t.dst = mats[i].dst; t.rows = mats[i].rows; t.cols = mats[i].cols;
@@ -320,14 +447,18 @@ int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out) {
         t.n = t.rows < t.cols ? t.cols : t.rows;
         t.ldx = (t.n + 7) / 8 * 8;
         t.lda = (t.m + 7) / 8 * 8;
+        const long long parts = ((long long)t.rows * t.cols + OR_SUM - 1) / OR_SUM, tm = (t.m + lay.tb_sym - 1) / lay.tb_sym, ts = tm * (tm + 1) / 2;
+        const long long xm = (t.m + lay.tb_x - 1) / lay.tb_x, xn = (t.ldx + lay.tb_x - 1) / lay.tb_x;
+        long long sp = pieces < t.ldx / 512 ? pieces : t.ldx / 512;
+        if (sp < 1) sp = 1;
+        t.chunk = (int)aadg_align_up((size_t)((t.ldx + sp - 1) / sp), OR_BK);
+        t.splits = (t.ldx + t.chunk - 1) / t.chunk;
+        lay.split = lay.split || t.splits > 1;
         const size_t px = aadg_align_up((size_t)3 * t.m * t.ldx * 2, 256), pa = aadg_align_up((size_t)3 * t.m * t.lda * 2, 256);
-        const long long parts = ((long long)t.rows * t.cols + OR_SUM - 1) / OR_SUM, tm = (t.m + lay.tb - 1) / lay.tb, tn = (t.ldx + lay.tb - 1) / lay.tb;
-        t.x0 = (long long)at; at += px;
-        t.x1 = (long long)at; at += px;
-        t.a = (long long)at; at += pa;
-        t.b = (long long)at; at += pa;
+        for (int b = 0; b < OR_BUFS; ++b) { t.buf[b] = (long long)at; at += b == OR_B_X0 || b == OR_B_X1 ? px : pa; }
         t.sums = (long long)at; at += aadg_align_up((size_t)parts * 8, 256);
-        const long long wgs[OR_PHASES] = {parts, (long long)((t.m + 31) / 32) * ((t.ldx + 31) / 32), tm * (tm + 1) / 2, tm * tn};
+        t.part = (long long)at; at += t.splits > 1 ? (size_t)ts * t.splits * lay.tb_sym * lay.tb_sym * 4 : 0;
+        const long long wgs[OR_PHASES] = {parts, (long long)((t.m + 31) / 32) * ((t.ldx + 31) / 32), ts * t.splits, ts, xm * xn};
         for (int p = 0; p < OR_PHASES; ++p) {
             t.first[p] = (int)lay.grid[p];
             lay.grid[p] += wgs[p];
@@ -339,11 +470,66 @@ int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out) {
     return 0;
 }
 
-template <int TB> int or_steps(const OrLayout& lay, const OrMat* table, int n, int steps, float a, float b, float c, char* ws, hipStream_t st) {
-    for (int s = 0; s < steps; ++s) {
-        hipLaunchKernelGGL((k_or_mul<OR_A, TB>), dim3((unsigned)lay.grid[OR_P_SYM]), dim3(256), 0, st, table, n, ws, 0.0f, 0.0f, s & 1, 0);
-        hipLaunchKernelGGL((k_or_mul<OR_B, TB>), dim3((unsigned)lay.grid[OR_P_SYM]), dim3(256), 0, st, table, n, ws, b, c, s & 1, 0);
-        hipLaunchKernelGGL((k_or_mul<OR_X, TB>), dim3((unsigned)lay.grid[OR_P_X]), dim3(256), 0, st, table, n, ws, a, 0.0f, s & 1, s == steps - 1);
+struct OrRun {
+    const OrLayout& lay;
+    const OrMat* table;
+    int n;
+    char* ws;
+    hipStream_t st;
+    void gram(int x) const {
+        const OrOps o = {{{x, x, OR_B_A, -1, 1.0f, 0.0f, 0.0f}}};
+        const dim3 grid((unsigned)lay.grid[OR_P_GRAM]), join((unsigned)lay.grid[OR_P_SYM]);
+        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_mul<OR_GRAM, 128>), grid, dim3(256), 0, st, table, n, ws, o, 0);
+        else hipLaunchKernelGGL((k_or_mul<OR_GRAM, 64>), grid, dim3(256), 0, st, table, n, ws, o, 0);
+        if (!lay.split) return;
+        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_reduce<128>), join, dim3(256), 0, st, table, n, ws, o);
+        else hipLaunchKernelGGL((k_or_reduce<64>), join, dim3(256), 0, st, table, n, ws, o);
+    }
+    void sym(const OrOps& o, int count) const {
+        const dim3 grid((unsigned)lay.grid[OR_P_SYM], (unsigned)count);
+        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_mul<OR_SYM, 128>), grid, dim3(256), 0, st, table, n, ws, o, 0);
+        else hipLaunchKernelGGL((k_or_mul<OR_SYM, 64>), grid, dim3(256), 0, st, table, n, ws, o, 0);
+    }
+    void sym(OrOp a) const { sym(OrOps{{a, a}}, 1); }
+    void apply(int l, int x, int y, bool last) const {
+        const OrOps o = {{{l, x, y, -1, 1.0f, 0.0f, 0.0f}}};
+        const dim3 grid((unsigned)lay.grid[OR_P_X]);
+        if (lay.tb_x == 128) hipLaunchKernelGGL((k_or_mul<OR_X, 128>), grid, dim3(256), 0, st, table, n, ws, o, last);
+        else hipLaunchKernelGGL((k_or_mul<OR_X, 64>), grid, dim3(256), 0, st, table, n, ws, o, last);
+    }
+};
+
+int or_steps(const OrRun& run, int steps, float a, float b, float c) {
+    int x = OR_B_X0, y = OR_B_X1;
+    for (int done = 0; done < steps;) {
+        const int block = steps - done < (done == 0 ? 2 : 3) ? steps - done : (done == 0 ? 2 : 3);
+        done += block;
+        run.gram(x);
+        int p = OR_B_P0, p2 = OR_B_P1, q = -1, free_q = OR_B_Q;                // q: the product of the block's P so far
+        for (int k = 0; k < block; ++k) {
+            run.sym({OR_B_A, OR_B_A, p, OR_B_A, c, b, a});                    // P = a I + b A + c A A
+            const OrOp fold = {p, q, q < 0 ? -1 : (q == OR_B_Q ? OR_B_T : free_q), -1, 1.0f, 0.0f, 0.0f};        // Q <- P Q
+            const OrOp half = {p, OR_B_A, OR_B_T, -1, 1.0f, 0.0f, 0.0f};       // T = P A
+            const bool more = k + 1 < block;
+            if (q < 0) {
+                if (more) run.sym(half);
+                q = p;
+            } else if (more) {
+                run.sym(OrOps{{half, fold}}, 2);
+                q = fold.o;
+            } else {
+                run.sym(fold);
+                q = fold.o;
+            }
+            if (more) run.sym({OR_B_T, p, OR_B_A, -1, 1.0f, 0.0f, 0.0f});      // A <- P A P
+            const int s = p;
+            p = p2;
+            p2 = s;
+        }
+        run.apply(q, x, y, done == steps);
+        const int s = x;
+        x = y;
+        y = s;
         AADG_LAUNCH_CHECK();
     }
     return 0;
@@ -384,5 +570,5 @@ extern "C" int aadg_orthogonalize_f32(const aadg_matrix* mats_host, int n, int s
     hipLaunchKernelGGL(k_or_sum, dim3((unsigned)lay.grid[OR_P_SUM]), dim3(256), 0, st, table, n, (char*)ws);
     hipLaunchKernelGGL(k_or_planes, dim3((unsigned)lay.grid[OR_P_SPLIT]), dim3(256), 0, st, table, n, (char*)ws, eps);
     AADG_LAUNCH_CHECK();
-    return lay.tb == 128 ? or_steps<128>(lay, table, n, steps, a, b, c, (char*)ws, st) : or_steps<64>(lay, table, n, steps, a, b, c, (char*)ws, st);
+    return or_steps(OrRun{lay, table, n, (char*)ws, st}, steps, a, b, c);
 }
