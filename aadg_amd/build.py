@@ -22,9 +22,9 @@ HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-cont
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                "-Wall", "-Wno-unused-function", "-I" + INCLUDE, "-I" + CSRC]
 
-# accumulators in ordinary registers: where vector code touches every product (the softmax, its gradient) the default, accumulation registers,
+# accumulators in ordinary registers: where vector code touches every product (the softmax, its gradient, sums kept outside the matrix unit) the default, accumulation registers,
 # costs a move per value and direction
-SOURCE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+SOURCE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"], "orthogonalize.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _hipcc():

@@ -12,6 +12,8 @@
 //
 // All matrices of the list go through each phase in ONE launch: a workgroup finds its matrix from the running tile counts of a table in the
 // workspace.  The table travels in kernel arguments (26 entries a launch), so a captured graph keeps it.
+#include <algorithm>
+
 #include "common.h"
 
 namespace {
@@ -22,7 +24,8 @@ typedef short or_v4i16 __attribute__((ext_vector_type(4)));
 typedef short or_v8i16 __attribute__((ext_vector_type(8)));
 typedef uint32_t or_u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int OR_BK = 32;                             // contracted values per LDS stage
+constexpr int OR_NT = 512;                            // threads of a product workgroup
+constexpr int OR_PAD = 64;                            // leading dimensions of the planes: multiples of it, zero-filled (the longest LDS stage)
 constexpr int OR_SUM = 16384;                         // elements per workgroup of the norm
 constexpr int OR_CHUNK = 26;                          // table entries per launch (kernel arguments: 4 KB)
 
@@ -45,6 +48,17 @@ __global__ void k_or_table(const OrChunk c, OrMat* __restrict__ table) {
     const int* s = reinterpret_cast<const int*>(c.mat);
     int* d = reinterpret_cast<int*>(table + c.base);
     for (int i = threadIdx.x; i < words; i += blockDim.x) d[i] = s[i];
+}
+
+// Workgroups are dealt to the eight dies in turn, each with an L2 of its own: die x takes every eighth group of OR_GROUP neighbouring tiles, so
+// tiles that read the same rows mostly share an L2 (tile by tile over all dies the loads of a stage took longer than its products: 12 TB/s
+// past the L2s); whole eighths of the list per die left the dies unequal work.
+constexpr int OR_GROUP = 8;
+__device__ __forceinline__ int or_tile() {
+    const int w = blockIdx.x, whole = gridDim.x / (8 * OR_GROUP) * (8 * OR_GROUP);
+    if (w >= whole) return w;
+    const int i = w >> 3;
+    return ((i / OR_GROUP) * 8 + (w & 7)) * OR_GROUP + i % OR_GROUP;
 }
 
 // the matrix workgroup `wg` of phase `ph` belongs to: the last one whose first workgroup is not behind it (one wave, 64 entries at a time)
@@ -128,8 +142,8 @@ __global__ __launch_bounds__(256) void k_or_planes(const OrMat* __restrict__ tab
     }
 }
 
-// LDS layouts.  K-contiguous operand: rows of OR_BK values, chunk c of row r at c ^ ((r >> 2) & 3): 8 rows of one chunk hit all banks.
-__device__ __forceinline__ int or_row_at(int row, int chunk) { return row * OR_BK + ((chunk ^ ((row >> 2) & 3)) << 3); }
+// LDS layouts.  K-contiguous operand: rows of BK values, the 16-byte chunks of a row permuted such that 8 rows of one chunk hit all banks.
+template <int BK> __device__ __forceinline__ int or_row_at(int row, int chunk) { return row * BK + ((chunk ^ (BK == 32 ? (row >> 2) & 3 : (((row >> 1) & 1) << 2) | ((row >> 2) & 3))) << 3); }
 // K-strided operand ([k][TB] as in memory): chunks permuted such that the 4 rows x 4 chunks of a transpose read hit all banks
 template <int TB> __device__ __forceinline__ int or_col_at(int k, int chunk) {
     return k * TB + ((chunk ^ (TB == 128 ? ((k & 3) << 2) | ((k >> 2) & 3) : (((k >> 1) & 1) << 2) | ((k >> 2) & 3))) << 3);
@@ -193,7 +207,7 @@ __device__ __forceinline__ void or_store_symmetric(const OrMat& t, const float* 
     const uint16_t* E = op.e < 0 ? nullptr : reinterpret_cast<const uint16_t*>(ws + t.buf[op.e]);
     const int i0 = ti * TB, j0 = tj * TB;
 #pragma unroll 2
-    for (int id = threadIdx.x; id < TB * C8; id += 256) {
+    for (int id = threadIdx.x; id < TB * C8; id += OR_NT) {
         const int r = id / C8, c = (id - r * C8) * 8, row = i0 + r, col = j0 + c;
         if (row >= m || col >= lda) continue;
         float v[8], e[8];
@@ -208,11 +222,13 @@ __device__ __forceinline__ void or_store_symmetric(const OrMat& t, const float* 
 #pragma unroll
             for (int x = 0; x < 8; ++x) v[x] += row == col + x ? op.cd : 0.0f;
         }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = col + x < m ? v[x] : 0.0f;
         or_store8(out + (long long)row * lda + col, plane, v);
     }
     if (ti == tj) return;
 #pragma unroll 2
-    for (int id = threadIdx.x; id < TB * C8; id += 256) {                    // mirrored row = the tile's column: neighbouring lanes, neighbouring columns
+    for (int id = threadIdx.x; id < TB * C8; id += OR_NT) {                  // mirrored row = the tile's column: neighbouring lanes, neighbouring columns
         const int r8 = id / TB * 8, c = id - id / TB * TB, row = j0 + c, col = i0 + r8;
         if (row >= m || col >= lda) continue;
         float v[8], e[8];
@@ -223,27 +239,33 @@ __device__ __forceinline__ void or_store_symmetric(const OrMat& t, const float* 
 #pragma unroll
             for (int x = 0; x < 8; ++x) v[x] = fmaf(op.cb, e[x], v[x]);
         }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = col + x < m ? v[x] : 0.0f;
         or_store8(out + (long long)row * lda + col, plane, v);
     }
 }
 
-// One TB x TB tile of a product, 4 waves of (TB / 2) x (TB / 2).
+// One TB x TB tile of a product, 8 waves: 128: 64 x 32 each, stages of 32 values; 64: 32 x 32 each, two groups of four waves on the two
+// halves of stages of 64 values (their sums meet in the tile).
 //   PH = OR_GRAM: L = R = X (K = n, cut into t.splits pieces; more than one: the partial tile goes to the workspace for k_or_reduce), symmetric
 //   PH = OR_SYM:  L, R symmetric matrices that commute, the product symmetric
 //   PH = OR_X:    L symmetric, R = X, the K-strided operand (transpose reads); `last`: the result goes to the caller's matrix
-// Of a symmetric product the tiles tj <= ti are computed and stored twice.
+// Of a symmetric product the tiles tj <= ti are computed and stored twice.  The lists are a few hundred tiles, a workgroup mostly has its CU for
+// itself: two LDS buffers, one barrier a stage, the loads of the stage after the next in flight during the products.  Rows outside the
+// matrix are read from its last row (their results are not stored); the contracted axis ends in zeros.
 enum { OR_GRAM, OR_SYM, OR_X };
 template <int PH, int TB>
-__global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table, int count, char* __restrict__ ws, const OrOps ops, int last) {
-    constexpr int W = TB / 64, LR = 3 * TB * (OR_BK / 8) / 256;             // 32-wide blocks per wave side; 16-byte chunks per thread and operand
-    constexpr int TP = TB + 8, STAGE = 2 * 3 * TB * OR_BK * 2, BYTES = STAGE > TB * TP * 4 ? STAGE : TB * TP * 4;
+__global__ __launch_bounds__(OR_NT, 2) void k_or_mul(const OrMat* __restrict__ table, int count, char* __restrict__ ws, const OrOps ops, int last) {
+    constexpr int BK = TB == 128 ? 32 : 64, CPR = BK / 8, WX = TB / 64, LR = 3 * TB * CPR / OR_NT;      // WX: 32-row blocks per wave; 16-byte chunks per thread and operand
+    constexpr int TP = TB + 8, OPND = 3 * TB * BK, STAGE = 2 * OPND * 2, BYTES = 2 * STAGE > TB * TP * 4 ? 2 * STAGE : TB * TP * 4;
     __shared__ __attribute__((aligned(16))) char lds[BYTES];
-    uint16_t *Ls = reinterpret_cast<uint16_t*>(lds), *Rs = Ls + 3 * TB * OR_BK;
+    uint16_t* buf = reinterpret_cast<uint16_t*>(lds);                       // [2 stages][L, R][3 planes]
     constexpr int PHASE = PH == OR_GRAM ? OR_P_GRAM : PH == OR_SYM ? OR_P_SYM : OR_P_X;
-    const OrMat& t = table[or_find(table, count, PHASE, blockIdx.x)];
+    const int wg = or_tile();
+    const OrMat& t = table[or_find(table, count, PHASE, wg)];
     const OrOp op = ops.op[blockIdx.y];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = lane >> 5;
-    int w = blockIdx.x - t.first[PHASE], ti, tj, k_lo = 0, sp = 0;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    int w = wg - t.first[PHASE], ti, tj, k_lo = 0, sp = 0;
     const uint16_t* L = reinterpret_cast<const uint16_t*>(ws + t.buf[op.l]);
     const uint16_t* R = reinterpret_cast<const uint16_t*>(ws + t.buf[op.r]);
     const int m = t.m, ldl = PH == OR_GRAM ? t.ldx : t.lda, ldr = PH == OR_SYM ? t.lda : t.ldx;
@@ -262,100 +284,121 @@ __global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table,
         or_triangle(w, ti, tj);
     }
     const long long pl_l = (long long)m * ldl, pl_r = (long long)m * ldr;
-    const int i0 = ti * TB, j0 = tj * TB, wi = (wv >> 1) * (TB / 2), wj = (wv & 1) * (TB / 2);
+    const int i0 = ti * TB, j0 = tj * TB;
+    const int wi = TB == 128 ? (wv >> 2) * 64 : (wv & 2) * 16, wj = TB == 128 ? (wv & 3) * 32 : (wv & 1) * 32, u0 = TB == 128 ? 0 : (wv >> 2) * 2;
 
-    uint4 rl[LR], rr[LR];
-    auto fetch = [&](int k0) {
+    struct Regs { or_u32x4 l[LR], r[LR]; } ra, rb;                           // two stages under way
+    auto fetch = [&](Regs& g, int k0) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < LR; ++i) {
-            const int id = tid + 256 * i;
-            {
-                const int pl = id / (TB * 4), q = id - pl * (TB * 4), row = i0 + (q >> 2), k = k0 + (q & 3) * 8;
-                const uint4 x = *reinterpret_cast<const uint4*>(L + pl * pl_l + (long long)min(row, m - 1) * ldl + min(k, ldl - 8));
-                rl[i] = row < m && k < ldl ? x : make_uint4(0, 0, 0, 0);
-            }
+            const int id = tid + OR_NT * i;
+            const int pl = id / (TB * CPR), q = id - pl * (TB * CPR), c = k0 + (q % CPR) * 8;
+            g.l[i] = *reinterpret_cast<const or_u32x4*>(L + pl * pl_l + (long long)min(i0 + q / CPR, m - 1) * ldl + c);
             if (PH != OR_X) {
-                const int pl = id / (TB * 4), q = id - pl * (TB * 4), row = j0 + (q >> 2), k = k0 + (q & 3) * 8;
-                const uint4 x = *reinterpret_cast<const uint4*>(R + pl * pl_r + (long long)min(row, m - 1) * ldr + min(k, ldr - 8));
-                rr[i] = row < m && k < ldr ? x : make_uint4(0, 0, 0, 0);
+                g.r[i] = *reinterpret_cast<const or_u32x4*>(R + pl * pl_r + (long long)min(j0 + q / CPR, m - 1) * ldr + c);
             } else {
-                const int pl = id / (OR_BK * (TB / 8)), q = id - pl * (OR_BK * (TB / 8)), k = k0 + q / (TB / 8), c = j0 + (q % (TB / 8)) * 8;
-                const uint4 x = *reinterpret_cast<const uint4*>(R + pl * pl_r + (long long)min(k, m - 1) * ldr + min(c, ldr - 8));
-                rr[i] = k < m && c < ldr ? x : make_uint4(0, 0, 0, 0);
+                const int pr = id / (BK * (TB / 8)), s = id - pr * (BK * (TB / 8));
+                g.r[i] = *reinterpret_cast<const or_u32x4*>(R + pr * pl_r + (long long)min(k0 + s / (TB / 8), m - 1) * ldr + min(j0 + (s % (TB / 8)) * 8, ldr - 8));
             }
         }
     };
-    f32x16 acc[W][W];
-#pragma unroll
-    for (int x = 0; x < W; ++x)
-#pragma unroll
-        for (int y = 0; y < W; ++y)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[x][y][i] = 0.0f;
-    fetch(k_lo);
-    for (int k0 = k_lo; k0 < K; k0 += OR_BK) {
-        __syncthreads();
+    auto stage = [&](const Regs& g, int b) __attribute__((always_inline)) {
+        uint16_t *Ls = buf + b * 2 * OPND, *Rs = Ls + OPND;
 #pragma unroll
         for (int i = 0; i < LR; ++i) {
-            const int id = tid + 256 * i;
-            {
-                const int pl = id / (TB * 4), q = id - pl * (TB * 4);
-                *reinterpret_cast<uint4*>(&Ls[pl * TB * OR_BK + or_row_at(q >> 2, q & 3)]) = rl[i];
-                if (PH != OR_X) *reinterpret_cast<uint4*>(&Rs[pl * TB * OR_BK + or_row_at(q >> 2, q & 3)]) = rr[i];
-            }
-            if (PH == OR_X) {
-                const int pl = id / (OR_BK * (TB / 8)), q = id - pl * (OR_BK * (TB / 8));
-                *reinterpret_cast<uint4*>(&Rs[pl * TB * OR_BK + or_col_at<TB>(q / (TB / 8), q % (TB / 8))]) = rr[i];
+            const int id = tid + OR_NT * i;
+            const int pl = id / (TB * CPR), q = id - pl * (TB * CPR), at = pl * TB * BK + or_row_at<BK>(q / CPR, q % CPR);
+            *reinterpret_cast<or_u32x4*>(&Ls[at]) = g.l[i];
+            if (PH != OR_X) {
+                *reinterpret_cast<or_u32x4*>(&Rs[at]) = g.r[i];
+            } else {
+                const int pr = id / (BK * (TB / 8)), s = id - pr * (BK * (TB / 8));
+                *reinterpret_cast<or_u32x4*>(&Rs[pr * TB * BK + or_col_at<TB>(s / (TB / 8), s % (TB / 8))]) = g.r[i];
             }
         }
-        __syncthreads();
-        if (k0 + OR_BK < K) fetch(k0 + OR_BK);
+    };
+    f32x16 acc[WX];
 #pragma unroll
-        for (int u = 0; u < OR_BK / 16; ++u) {
-            or_bf16x8 l[3][W], r[3][W];
+    for (int x = 0; x < WX; ++x)
 #pragma unroll
-            for (int p = 0; p < 3; ++p)
+        for (int i = 0; i < 16; ++i) acc[x][i] = 0.0f;
+    auto multiply = [&](int b) __attribute__((always_inline)) {
+        const uint16_t *Ls = buf + b * 2 * OPND, *Rs = Ls + OPND;
 #pragma unroll
-                for (int x = 0; x < W; ++x) {
-                    l[p][x] = __builtin_bit_cast(or_bf16x8, *reinterpret_cast<const or_u32x4*>(&Ls[p * TB * OR_BK + or_row_at(wi + 32 * x + (lane & 31), 2 * u + h)]));
-                    if (PH != OR_X)
-                        r[p][x] = __builtin_bit_cast(or_bf16x8, *reinterpret_cast<const or_u32x4*>(&Rs[p * TB * OR_BK + or_row_at(wj + 32 * x + (lane & 31), 2 * u + h)]));
-                    else
-                        r[p][x] = or_cols<TB>(&Rs[p * TB * OR_BK], 16 * u, wj + 32 * x, lane);
-                }
+        for (int v = 0; v < 2; ++v) {
+            const int u = u0 + v;
+            or_bf16x8 l[3][WX], r[3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+#pragma unroll
+                for (int x = 0; x < WX; ++x)
+                    l[p][x] = __builtin_bit_cast(or_bf16x8, *reinterpret_cast<const or_u32x4*>(&Ls[p * TB * BK + or_row_at<BK>(wi + 32 * x + (lane & 31), 2 * u + h)]));
+                if (PH != OR_X) r[p] = __builtin_bit_cast(or_bf16x8, *reinterpret_cast<const or_u32x4*>(&Rs[p * TB * BK + or_row_at<BK>(wj + (lane & 31), 2 * u + h)]));
+                else r[p] = or_cols<TB>(&Rs[p * TB * BK], 16 * u, wj, lane);
+            }
             // weights 2^-16, 2^-8, 1: the small ones first.  The six start from zero and their sum is added to the accumulator by the vector
             // unit: accumulating in the matrix instruction rounds 6 K / 16 times at the size of the whole sum and with a bias (3.7e-6
             // instead of 6e-7 of the result at K = 768)
+            f32x16 d[WX] = {};
 #pragma unroll
-            for (int x = 0; x < W; ++x)
+            for (int x = 0; x < WX; ++x) d[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[2][x], r[0], d[x], 0, 0, 0);
 #pragma unroll
-                for (int y = 0; y < W; ++y) {
-                    f32x16 d = {};
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[2][x], r[0][y], d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[2][y], d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[1][x], r[1][y], d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[1][x], r[0][y], d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[1][y], d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[0][y], d, 0, 0, 0);
+            for (int x = 0; x < WX; ++x) d[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[2], d[x], 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[x][y][i] += d[i];
-                }
+            for (int x = 0; x < WX; ++x) d[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[1][x], r[1], d[x], 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < WX; ++x) d[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[1][x], r[0], d[x], 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < WX; ++x) d[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[1], d[x], 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < WX; ++x) d[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l[0][x], r[0], d[x], 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < WX; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[x][i] += d[x][i];
         }
+    };
+    // stage s is multiplied while s + 1 goes to the other buffer and s + 2, s + 3 are on their way (a trip past the L2, where the last phase's
+    // workgroups of other dies left the data, takes longer than a stage's products); behind the end the last stage is read again, unused
+    const int last_k = K - BK;
+    fetch(ra, k_lo);
+    fetch(rb, min(k_lo + BK, last_k));
+    stage(ra, 0);
+    __builtin_amdgcn_sched_barrier(0);                                        // (loads in the order in which the loop waits for them)
+    fetch(ra, min(k_lo + 2 * BK, last_k));
+    __syncthreads();
+    int k0 = k_lo;
+    for (; k0 + BK < K; k0 += 2 * BK) {
+        stage(rb, 1);
+        fetch(rb, min(k0 + 3 * BK, last_k));
+        multiply(0);
+        __syncthreads();
+        stage(ra, 0);
+        fetch(ra, min(k0 + 4 * BK, last_k));
+        multiply(1);
+        __syncthreads();
     }
+    if (k0 < K) multiply(0);
+    __syncthreads();
     // the tile goes through LDS (register i of half h = row 8 (i / 4) + 4 h + i % 4, lane & 31 = column: 2-byte stores of the planes straight from
     // the registers took longer than the product): pitch TB + 8 words, the two halves of a write 32 banks apart
     float* tile = reinterpret_cast<float*>(lds);
-    __syncthreads();
 #pragma unroll
-    for (int x = 0; x < W; ++x)
+    for (int g = 0; g < (TB == 128 ? 1 : 2); ++g) {
+        if (TB == 128 || (wv >> 2) == g) {
 #pragma unroll
-        for (int y = 0; y < W; ++y)
+            for (int x = 0; x < WX; ++x)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) tile[(wi + 32 * x + 8 * (i >> 2) + 4 * h + (i & 3)) * TP + wj + 32 * y + (lane & 31)] = acc[x][y][i];
-    __syncthreads();
+                for (int i = 0; i < 16; ++i) {
+                    float& at = tile[(wi + 32 * x + 8 * (i >> 2) + 4 * h + (i & 3)) * TP + wj + (lane & 31)];
+                    at = g == 0 ? acc[x][i] : at + acc[x][i];
+                }
+        }
+        __syncthreads();
+    }
     if (PH == OR_GRAM && t.splits > 1) {
         float4* part = reinterpret_cast<float4*>(ws + t.part) + ((long long)w * t.splits + sp) * (TB * TB / 4);
-        for (int id = tid; id < TB * TB / 4; id += 256) {
+        for (int id = tid; id < TB * TB / 4; id += OR_NT) {
             const int r = id / (TB / 4), c = (id - r * (TB / 4)) * 4;
             part[id] = *reinterpret_cast<const float4*>(&tile[r * TP + c]);
         }
@@ -367,9 +410,9 @@ __global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table,
     }
     if (!last) {
         uint16_t* out = reinterpret_cast<uint16_t*>(ws + t.buf[op.o]);
-        for (int id = tid; id < TB * (TB / 8); id += 256) {
+        for (int id = tid; id < TB * (TB / 8); id += OR_NT) {
             const int r = id / (TB / 8), c = (id - r * (TB / 8)) * 8;
-            if (i0 + r >= t.m || j0 + c >= t.ldx) continue;
+            if (i0 + r >= m || j0 + c >= t.ldx) continue;
             float v[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) v[x] = tile[r * TP + c + x];
@@ -378,24 +421,25 @@ __global__ __launch_bounds__(256) void k_or_mul(const OrMat* __restrict__ table,
         return;
     }
     const bool tall = t.rows > t.cols;
-    for (int id = tid; id < TB * TB; id += 256) {                             // lanes along the rows of the caller's matrix
+    for (int id = tid; id < TB * TB; id += OR_NT) {                             // lanes along the rows of the caller's matrix
         const int x = id / TB, y = id - x * TB, r = tall ? y : x, c = tall ? x : y;
-        if (i0 + r < t.m && j0 + c < t.n) t.dst[tall ? (long long)(j0 + c) * t.cols + i0 + r : (long long)(i0 + r) * t.cols + j0 + c] = tile[r * TP + c];
+        if (i0 + r < m && j0 + c < t.n) t.dst[tall ? (long long)(j0 + c) * t.cols + i0 + r : (long long)(i0 + r) * t.cols + j0 + c] = tile[r * TP + c];
     }
 }
 
 // joins the pieces of the long products A = X X^T in order
 template <int TB>
-__global__ __launch_bounds__(256) void k_or_reduce(const OrMat* __restrict__ table, int count, char* __restrict__ ws, const OrOps ops) {
+__global__ __launch_bounds__(OR_NT) void k_or_reduce(const OrMat* __restrict__ table, int count, char* __restrict__ ws, const OrOps ops) {
     constexpr int TP = TB + 8;
     __shared__ __attribute__((aligned(16))) float tile[TB * TP];
-    const OrMat& t = table[or_find(table, count, OR_P_SYM, blockIdx.x)];
+    const int wg = or_tile();
+    const OrMat& t = table[or_find(table, count, OR_P_SYM, wg)];
     if (t.splits == 1) return;                                                // (stored by the product itself)
-    const int w = blockIdx.x - t.first[OR_P_SYM];
+    const int w = wg - t.first[OR_P_SYM];
     int ti, tj;
     or_triangle(w, ti, tj);
     const float4* part = reinterpret_cast<const float4*>(ws + t.part) + (long long)w * t.splits * (TB * TB / 4);
-    for (int id = threadIdx.x; id < TB * TB / 4; id += 256) {
+    for (int id = threadIdx.x; id < TB * TB / 4; id += OR_NT) {
         float4 s = part[id];
 #pragma unroll 4
         for (int k = 1; k < t.splits; ++k) {
@@ -414,8 +458,18 @@ constexpr int OR_MAX_SIDE = 1 << 16, OR_MAX_MATS = 4096;
 
 struct OrLayout { size_t bytes; long long grid[OR_PHASES]; int tb_sym, tb_x; bool split; };
 
-// 0 or an error; fills the entries if `out` is given (n entries)
-int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out) {
+// The order of the table: most work first.  order: n entries
+int64_t or_work(const aadg_matrix& a) {
+    const int64_t m = a.rows < a.cols ? a.rows : a.cols;
+    return m * ((int64_t)a.rows * a.cols + m * m);
+}
+void or_order(const aadg_matrix* mats, int n, int* order) {
+    for (int i = 0; i < n; ++i) order[i] = i;
+    std::sort(order, order + n, [&](int x, int y) { return or_work(mats[x]) != or_work(mats[y]) ? or_work(mats[x]) > or_work(mats[y]) : x < y; });
+}
+
+// 0 or an error; fills the entries if `out` is given (n entries, matrix order[i] at i)
+int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out, const int* order) {
     if (mats == nullptr || n < 1 || n > OR_MAX_MATS) return AADG_E_BADARG;
     for (int i = 0; i < n; ++i) {
         if (mats[i].rows < 1 || mats[i].cols < 1) return AADG_E_BADARG;
@@ -441,17 +495,18 @@ int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out) {
     for (int p = 0; p < OR_PHASES; ++p) lay.grid[p] = 0;
     lay.split = false;
     for (int i = 0; i < n; ++i) {
+        const aadg_matrix& a = mats[order != nullptr ? order[i] : i];
         OrMat t = {};
-        t.src = mats[i].src; t.dst = mats[i].dst; t.rows = mats[i].rows; t.cols = mats[i].cols;
+        t.src = a.src; t.dst = a.dst; t.rows = a.rows; t.cols = a.cols;
         t.m = t.rows < t.cols ? t.rows : t.cols;
         t.n = t.rows < t.cols ? t.cols : t.rows;
-        t.ldx = (t.n + 7) / 8 * 8;
-        t.lda = (t.m + 7) / 8 * 8;
+        t.ldx = (t.n + OR_PAD - 1) / OR_PAD * OR_PAD;
+        t.lda = (t.m + OR_PAD - 1) / OR_PAD * OR_PAD;
         const long long parts = ((long long)t.rows * t.cols + OR_SUM - 1) / OR_SUM, tm = (t.m + lay.tb_sym - 1) / lay.tb_sym, ts = tm * (tm + 1) / 2;
         const long long xm = (t.m + lay.tb_x - 1) / lay.tb_x, xn = (t.ldx + lay.tb_x - 1) / lay.tb_x;
         long long sp = pieces < t.ldx / 512 ? pieces : t.ldx / 512;
         if (sp < 1) sp = 1;
-        t.chunk = (int)aadg_align_up((size_t)((t.ldx + sp - 1) / sp), OR_BK);
+        t.chunk = (int)aadg_align_up((size_t)((t.ldx + sp - 1) / sp), OR_PAD);
         t.splits = (t.ldx + t.chunk - 1) / t.chunk;
         lay.split = lay.split || t.splits > 1;
         const size_t px = aadg_align_up((size_t)3 * t.m * t.ldx * 2, 256), pa = aadg_align_up((size_t)3 * t.m * t.lda * 2, 256);
@@ -479,23 +534,23 @@ struct OrRun {
     void gram(int x) const {
         const OrOps o = {{{x, x, OR_B_A, -1, 1.0f, 0.0f, 0.0f}}};
         const dim3 grid((unsigned)lay.grid[OR_P_GRAM]), join((unsigned)lay.grid[OR_P_SYM]);
-        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_mul<OR_GRAM, 128>), grid, dim3(256), 0, st, table, n, ws, o, 0);
-        else hipLaunchKernelGGL((k_or_mul<OR_GRAM, 64>), grid, dim3(256), 0, st, table, n, ws, o, 0);
+        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_mul<OR_GRAM, 128>), grid, dim3(OR_NT), 0, st, table, n, ws, o, 0);
+        else hipLaunchKernelGGL((k_or_mul<OR_GRAM, 64>), grid, dim3(OR_NT), 0, st, table, n, ws, o, 0);
         if (!lay.split) return;
-        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_reduce<128>), join, dim3(256), 0, st, table, n, ws, o);
-        else hipLaunchKernelGGL((k_or_reduce<64>), join, dim3(256), 0, st, table, n, ws, o);
+        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_reduce<128>), join, dim3(OR_NT), 0, st, table, n, ws, o);
+        else hipLaunchKernelGGL((k_or_reduce<64>), join, dim3(OR_NT), 0, st, table, n, ws, o);
     }
     void sym(const OrOps& o, int count) const {
         const dim3 grid((unsigned)lay.grid[OR_P_SYM], (unsigned)count);
-        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_mul<OR_SYM, 128>), grid, dim3(256), 0, st, table, n, ws, o, 0);
-        else hipLaunchKernelGGL((k_or_mul<OR_SYM, 64>), grid, dim3(256), 0, st, table, n, ws, o, 0);
+        if (lay.tb_sym == 128) hipLaunchKernelGGL((k_or_mul<OR_SYM, 128>), grid, dim3(OR_NT), 0, st, table, n, ws, o, 0);
+        else hipLaunchKernelGGL((k_or_mul<OR_SYM, 64>), grid, dim3(OR_NT), 0, st, table, n, ws, o, 0);
     }
     void sym(OrOp a) const { sym(OrOps{{a, a}}, 1); }
     void apply(int l, int x, int y, bool last) const {
         const OrOps o = {{{l, x, y, -1, 1.0f, 0.0f, 0.0f}}};
         const dim3 grid((unsigned)lay.grid[OR_P_X]);
-        if (lay.tb_x == 128) hipLaunchKernelGGL((k_or_mul<OR_X, 128>), grid, dim3(256), 0, st, table, n, ws, o, last);
-        else hipLaunchKernelGGL((k_or_mul<OR_X, 64>), grid, dim3(256), 0, st, table, n, ws, o, last);
+        if (lay.tb_x == 128) hipLaunchKernelGGL((k_or_mul<OR_X, 128>), grid, dim3(OR_NT), 0, st, table, n, ws, o, last);
+        else hipLaunchKernelGGL((k_or_mul<OR_X, 64>), grid, dim3(OR_NT), 0, st, table, n, ws, o, last);
     }
 };
 
@@ -539,22 +594,24 @@ int or_steps(const OrRun& run, int steps, float a, float b, float c) {
 
 extern "C" size_t aadg_orthogonalize_workspace_bytes(const aadg_matrix* mats_host, int n) {
     OrLayout lay;
-    return or_layout(mats_host, n, lay, nullptr) == 0 ? lay.bytes : 0;
+    return or_layout(mats_host, n, lay, nullptr, nullptr) == 0 ? lay.bytes : 0;
 }
 
 extern "C" int aadg_orthogonalize_f32(const aadg_matrix* mats_host, int n, int steps, float a, float b, float c, float eps, void* ws,
                                       size_t ws_bytes, void* stream) {
     OrLayout lay;
-    const int rc = or_layout(mats_host, n, lay, nullptr);
+    const int rc = or_layout(mats_host, n, lay, nullptr, nullptr);
     if (rc != 0) return rc;
     if (steps < 1 || steps > 64 || !(eps >= 0.0f)) return AADG_E_BADARG;
     for (int i = 0; i < n; ++i)
         if (mats_host[i].src == nullptr || mats_host[i].dst == nullptr || (uintptr_t)mats_host[i].src % 4 != 0 || (uintptr_t)mats_host[i].dst % 4 != 0)
             return AADG_E_BADARG;
     if (ws == nullptr || (uintptr_t)ws % 256 != 0 || ws_bytes < lay.bytes) return AADG_E_WORKSPACE;
-    OrMat* entries = (OrMat*)malloc((size_t)n * sizeof(OrMat));
+    OrMat* entries = (OrMat*)malloc((size_t)n * (sizeof(OrMat) + sizeof(int)));
     if (entries == nullptr) return AADG_E_WORKSPACE;
-    or_layout(mats_host, n, lay, entries);
+    int* order = (int*)(entries + n);
+    or_order(mats_host, n, order);
+    or_layout(mats_host, n, lay, entries, order);
     hipStream_t st = (hipStream_t)stream;
     OrMat* table = (OrMat*)ws;
     constexpr int PER = OR_CHUNK;
