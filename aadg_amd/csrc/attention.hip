@@ -51,6 +51,8 @@ struct AtArgs {
     int B, H, G, Nq, Nk, d, causal, r, R;
     int tiles, splits, chunk;                         // row (or key) tiles per group, splits of the loop axis, its length per split
     float scale;
+    unsigned mul;                                     // at_head
+    int shift;
 };
 
 template <typename T> struct At;
@@ -95,28 +97,28 @@ template <> struct At<float> {
     }
 };
 
-// A tile of rows x D in LDS, row-major.  bfloat16: no padding, the 16-byte chunks of a row permuted by a function of the row such that
-// both the row reads (8 rows, one chunk) and the transpose reads (4 rows, 4 neighbouring chunks) touch every bank once.
+// A tile of rows x D in LDS, row-major.  bfloat16: rows 16 banks (mod 64) apart, the four 16-byte chunks of a group permuted by the number of the
+// row's group of four: row reads (16 rows, one chunk) and transpose reads (4 rows, 4 neighbouring chunks) touch every bank once, and
+// because the permutation stays within four chunks a fragment's address is one of two registers and an immediate (a permutation of
+// whole rows took 40 address registers).
 // float32: pitch D + 8 words (row reads of 16 bytes: 8 banks apart; column reads: the two halves, 4 rows apart, 32 banks apart).
 template <typename T, int D> struct Tile;
 template <int D> struct Tile<uint16_t, D> {
-    static constexpr int PITCH = D;
-    static __device__ __forceinline__ int swz(int row) {
-        return D == 128 ? (((row & 3) << 2) | ((row >> 2) & 3)) : D == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : ((row >> 2) & 3);
-    }
-    static __device__ __forceinline__ int at(int row, int chunk) { return row * D + ((chunk ^ swz(row)) << 3); }
-    // rows row0 + (lane & 31), values KS u + 8 h .. + 7
+    static constexpr int PITCH = D == 32 ? 32 : D + 32;
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * PITCH + ((chunk ^ ((row >> 2) & 3)) << 3); }
+    // rows row0 + (lane & 31), values KS u + 8 h .. + 7; row0 a multiple of 16
     static __device__ __forceinline__ at_bf16x8 rows(const uint16_t* t, int row0, int u, int lane) {
-        return __builtin_bit_cast(at_bf16x8, *reinterpret_cast<const at_u32x4*>(t + at(row0 + (lane & 31), 2 * u + (lane >> 5))));
+        const uint16_t* base = t + (lane & 31) * PITCH + (((2 * (u & 1) + (lane >> 5)) ^ ((lane >> 2) & 3)) << 3);
+        return __builtin_bit_cast(at_bf16x8, *reinterpret_cast<const at_u32x4*>(base + row0 * PITCH + 32 * (u >> 1)));
     }
-    // column c0 + (lane & 31), rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3}: ds_read_b64_tr_b16 gives lane i of 16 the 4 rows of
-    // column i; the lane passes the address of row i / 4, columns 4 (i % 4)
+    // column c0 + (lane & 31), rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3}, row0 a multiple of 16, c0 of 32: ds_read_b64_tr_b16 gives
+    // lane i of 16 the 4 rows of column i; the lane passes the address of row i / 4, columns 4 (i % 4)
     static __device__ __forceinline__ at_bf16x8 cols(const uint16_t* t, int row0, int c0, int lane) {
-        const int i = lane & 15, row = row0 + 4 * (lane >> 5) + (i >> 2), c = c0 + (lane & 16) + 4 * (i & 3);
-        const uint16_t* p0 = t + at(row, c >> 3) + (c & 7);
-        const uint16_t* p1 = t + at(row + 8, c >> 3) + (c & 7);
+        const int i = lane & 15, h = lane >> 5, ch = ((lane >> 3) & 2) + ((i >> 1) & 1);
+        const uint16_t* p = t + (4 * h + (i >> 2)) * PITCH + 4 * (i & 1) + row0 * PITCH + c0;
         typedef at_v4i16 __attribute__((address_space(3)))* lds_p;
-        const at_v4i16 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p0)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p1));
+        const at_v4i16 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + ((ch ^ h) << 3)));
+        const at_v4i16 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + ((ch ^ h ^ 2) << 3) + 8 * PITCH));
         typedef short v8i16 __attribute__((ext_vector_type(8)));
         const v8i16 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         return __builtin_bit_cast(at_bf16x8, v);
@@ -134,21 +136,29 @@ template <int D> struct Tile<float, D> {
     }
 };
 
-// 16 bytes of row `row`, chunk c, of a strided matrix; zero outside rows < n, values < d (the address is clamped, never out of range)
-template <typename T>
-__device__ __forceinline__ uint4 at_load(const T* base, long long stride, int row, int n, int c, int d) {
-    const int col = c * At<T>::CH;
-    const bool ok = row < n && col < d;
-    const uint4 x = *reinterpret_cast<const uint4*>(base + (long long)(row < n ? row : n - 1) * stride + (col < d ? col : 0));
-    return ok ? x : make_uint4(0, 0, 0, 0);
+// 16 bytes of row `row` (clamped into 0 .. n - 1), chunk c (clamped into the d values) of a strided matrix; at_keep zeroes what does not exist.  Two
+// steps: the prefetched values are masked when they go to LDS, not where they are loaded (a select there waits for memory), and without a
+// branch per load.
+template <typename T> __device__ __forceinline__ at_u32x4 at_fetch(const T* base, long long stride, int row, int n, int c, int d) {
+    return *reinterpret_cast<const at_u32x4*>(base + (long long)min(row, n - 1) * stride + min(c * At<T>::CH, d - At<T>::CH));
 }
+__device__ __forceinline__ at_u32x4 at_keep(at_u32x4 x, bool ok) {
+    const uint32_t m = ok ? 0xFFFFFFFFu : 0u;
+    return x & at_u32x4{m, m, m, m};
+}
+template <typename T> __device__ __forceinline__ at_u32x4 at_load(const T* base, long long stride, int row, int n, int c, int d) {
+    return at_keep(at_fetch<T>(base, stride, row, n, c, d), row < n && c * At<T>::CH < d);
+}
+
+// head of a folded row within its group, row / Nq: the high half of row * mul, shifted (exact for row < 2^31: mul = ceil(2^(32 + shift) / Nq))
+__device__ __forceinline__ int at_head(const AtArgs& a, int row) { return a.r == 1 ? 0 : a.Nq == 1 ? row : (int)(__umulhi((unsigned)row, a.mul) >> a.shift); }
 
 // folded row -> element offset of a [B, H, Nq] strided matrix for group g
 __device__ __forceinline__ long long at_row(const AtArgs& a, const AtStride& s, int b, int g, int row) {
-    const int hr = a.r == 1 ? 0 : row / a.Nq, i = row - hr * a.Nq;
+    const int hr = at_head(a, row), i = row - hr * a.Nq;
     return b * s.b + (long long)(g * a.r + hr) * s.h + (long long)i * s.n;
 }
-__device__ __forceinline__ int at_query(const AtArgs& a, int row) { return a.r == 1 ? row : row % a.Nq; }
+__device__ __forceinline__ int at_query(const AtArgs& a, int row) { return row - at_head(a, row) * a.Nq; }
 
 __device__ __forceinline__ int at_len(const AtArgs& a, int b) {
     return a.key_lengths == nullptr ? a.Nk : max(0, min(a.Nk, a.key_lengths[b]));
@@ -163,7 +173,7 @@ __device__ __forceinline__ int at_limit(const AtArgs& a, int L, int row) {
 __device__ __forceinline__ int at_limit_max(const AtArgs& a, int L, int row0, int n) {
     const int last = min(row0 + n, a.R) - 1;
     if (!a.causal) return L;
-    if (a.r > 1 && row0 / a.Nq != last / a.Nq) return L;
+    if (at_head(a, row0) != at_head(a, last)) return L;
     return at_limit(a, L, last);
 }
 
@@ -214,13 +224,13 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_fwd(co
     float m = -INFINITY, l = 0.0f;
     const float c = a.scale * AT_LOG2E;
 
-    uint4 rk[LD], rv[LD];
+    at_u32x4 rk[LD], rv[LD];
     auto fetch = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
-            rk[i] = at_load<T>(kb, a.sk.n, k0 + rw, L, ch, a.d);
-            rv[i] = at_load<T>(vb, a.sv.n, k0 + rw, L, ch, a.d);
+            rk[i] = at_fetch<T>(kb, a.sk.n, k0 + rw, L, ch, a.d);
+            rv[i] = at_fetch<T>(vb, a.sv.n, k0 + rw, L, ch, a.d);
         }
     };
     if (k_lo < wg_end) fetch(k_lo);
@@ -229,8 +239,9 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_fwd(co
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
-            *reinterpret_cast<uint4*>(&Ks[L_::at(rw, ch)]) = rk[i];
-            *reinterpret_cast<uint4*>(&Vs[L_::at(rw, ch)]) = rv[i];
+            const bool ok = k0 + rw < L && ch * CH < a.d;
+            *reinterpret_cast<at_u32x4*>(&Ks[L_::at(rw, ch)]) = at_keep(rk[i], ok);
+            *reinterpret_cast<at_u32x4*>(&Vs[L_::at(rw, ch)]) = at_keep(rv[i], ok);
         }
         __syncthreads();
         if (k0 + BK < wg_end) fetch(k0 + BK);
@@ -426,13 +437,13 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
-    uint4 rk[LD], rv[LD];
+    at_u32x4 rk[LD], rv[LD];
     auto fetch = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
-            rk[i] = at_load<T>(kb, a.sk.n, k0 + rw, L, ch, a.d);
-            rv[i] = at_load<T>(vb, a.sv.n, k0 + rw, L, ch, a.d);
+            rk[i] = at_fetch<T>(kb, a.sk.n, k0 + rw, L, ch, a.d);
+            rv[i] = at_fetch<T>(vb, a.sv.n, k0 + rw, L, ch, a.d);
         }
     };
     if (k_lo < wg_end) fetch(k_lo);
@@ -441,8 +452,9 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
-            *reinterpret_cast<uint4*>(&Ks[L_::at(rw, ch)]) = rk[i];
-            *reinterpret_cast<uint4*>(&Vs[L_::at(rw, ch)]) = rv[i];
+            const bool ok = k0 + rw < L && ch * CH < a.d;
+            *reinterpret_cast<at_u32x4*>(&Ks[L_::at(rw, ch)]) = at_keep(rk[i], ok);
+            *reinterpret_cast<at_u32x4*>(&Vs[L_::at(rw, ch)]) = at_keep(rv[i], ok);
         }
         __syncthreads();
         if (k0 + BK < wg_end) fetch(k0 + BK);
@@ -492,7 +504,8 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
 }
 
 // dk, dv: a wave owns 32 keys (its K and V fragments stay in registers) and walks the folded rows, BQ at a time through LDS;
-// dv^T += dO^T P, dk^T += Q^T dS.  -D_i is the initial value of the dP accumulators.
+// dv^T += dO^T P, dk^T += Q^T dS.  -D_i is the initial value of the dP accumulators.  Head widths over 64 in bfloat16 keep V in LDS (32 KB) to stay
+// within 256 registers, two waves per SIMD: with one the walk is a chain of waits (MFMA busy 19 %).
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(const AtArgs a) {
     typedef At<T> M;
@@ -501,6 +514,8 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
     constexpr int LD = (BQ * CPR + NT - 1) / NT, DT = D / 32, PG = 16 / (KS / 2);
     __shared__ __attribute__((aligned(16))) T Qs[BQ * L_::PITCH];
     __shared__ __attribute__((aligned(16))) T Gs[BQ * L_::PITCH];
+    constexpr bool VL = false;
+    __shared__ __attribute__((aligned(16))) T Vs[VL ? 32 * NW * L_::PITCH : 8];
     __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
     __shared__ __attribute__((aligned(16))) int Es[BQ];                       // key limit of each row
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -513,12 +528,14 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
     const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
     const float c = a.scale * AT_LOG2E;
     const int r_lo = SPLIT ? sp * a.chunk : 0, r_hi = wg_key0 < L ? (SPLIT ? min(a.R, r_lo + a.chunk) : a.R) : r_lo;      // (no key: nothing to walk)
-    typename M::Frag kf[U], vf[U];
+    typename M::Frag kf[U], vf[VL ? 1 : U];
     if (wg_key0 < L) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             kf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(kb, a.sk.n, key, L, 2 * u + h, a.d));
-            vf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(vb, a.sv.n, key, L, 2 * u + h, a.d));
+            const at_u32x4 x = at_load<T>(vb, a.sv.n, key, L, 2 * u + h, a.d);
+            if (VL) *reinterpret_cast<at_u32x4*>(&Vs[L_::at(32 * wv + (lane & 31), 2 * u + h)]) = x;      // (read by this wave only)
+            else vf[u] = __builtin_bit_cast(typename M::Frag, x);
         }
     }
     f32x16 ak[DT], av[DT];
@@ -532,26 +549,18 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
             while (q0 < r_hi && at_limit_max(a, L, q0, BQ) <= wg_key0) q0 += BQ;
         return q0;
     };
-    uint4 rq[LD], rg[LD];
+    at_u32x4 rq[LD], rg[LD];
     float r_lse = 0.0f, r_d = 0.0f;
-    int r_lim = 0;
     auto fetch = [&](int q0) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR, rr = q0 + rw;
-            const bool ok = rr < r_hi && (BQ * CPR % NT == 0 || id < BQ * CPR);
-            const int rc = ok ? rr : q0;
-            rq[i] = at_load<T>((const T*)a.q + at_row(a, a.sq, b, g, rc), 0, ok ? 0 : 1, 1, ch, a.d);
-            rg[i] = at_load<T>((const T*)a.dout + at_row(a, a.sdo, b, g, rc), 0, ok ? 0 : 1, 1, ch, a.d);
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR, rr = min(q0 + rw, r_hi - 1);
+            rq[i] = at_fetch<T>((const T*)a.q + at_row(a, a.sq, b, g, rr), 0, 0, 1, ch, a.d);
+            rg[i] = at_fetch<T>((const T*)a.dout + at_row(a, a.sdo, b, g, rr), 0, 0, 1, ch, a.d);
         }
-        if (tid < BQ) {
-            const int rr = q0 + tid;
-            const bool ok = rr < r_hi;
-            const long long f = ((long long)b * a.G + g) * a.R + (ok ? rr : q0);
-            r_lse = ok ? a.lse[f] : INFINITY;
-            r_d = ok ? -a.delta[f] : 0.0f;
-            r_lim = ok ? at_limit(a, L, rr) : 0;
-        }
+        const long long f = ((long long)b * a.G + g) * a.R + min(q0 + (tid & (BQ - 1)), r_hi - 1);
+        r_lse = a.lse[f];
+        r_d = a.delta[f];
     };
     int q0 = next(r_lo);
     if (q0 < r_hi) fetch(q0);
@@ -561,13 +570,15 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
         for (int i = 0; i < LD; ++i) {
             const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
             if (BQ * CPR % NT != 0 && id >= BQ * CPR) break;
-            *reinterpret_cast<uint4*>(&Qs[L_::at(rw, ch)]) = rq[i];
-            *reinterpret_cast<uint4*>(&Gs[L_::at(rw, ch)]) = rg[i];
+            const bool ok = q0 + rw < r_hi && ch * CH < a.d;
+            *reinterpret_cast<at_u32x4*>(&Qs[L_::at(rw, ch)]) = at_keep(rq[i], ok);
+            *reinterpret_cast<at_u32x4*>(&Gs[L_::at(rw, ch)]) = at_keep(rg[i], ok);
         }
         if (tid < BQ) {
-            Ls[tid] = r_lse;
-            Ds[tid] = r_d;
-            Es[tid] = r_lim;
+            const bool ok = q0 + tid < r_hi;
+            Ls[tid] = ok ? r_lse : INFINITY;
+            Ds[tid] = ok ? -r_d : 0.0f;
+            Es[tid] = ok ? at_limit(a, L, q0 + tid) : 0;
         }
         __syncthreads();
         const int qn = next(q0 + BQ);
@@ -589,7 +600,7 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 s = M::mma(L_::rows(Qs, 32 * t, u, lane), kf[u], s);
-                dp = M::mma(L_::rows(Gs, 32 * t, u, lane), vf[u], dp);
+                dp = M::mma(L_::rows(Gs, 32 * t, u, lane), VL ? L_::rows(Vs, 32 * wv, u, lane) : vf[VL ? 0 : u], dp);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -727,6 +738,10 @@ void at_fill(AtArgs& a, const aadg_attention_desc* s, const int* key_lengths) {
     a.key_lengths = key_lengths;
     a.B = s->B; a.H = s->H; a.G = s->G; a.Nq = s->Nq; a.Nk = s->Nk; a.d = s->d; a.causal = s->causal != 0;
     a.r = s->H / s->G; a.R = a.r * s->Nq; a.scale = s->scale;
+    // 2^shift < Nq <= 2^(shift + 1): mul < 2^32, and mul * Nq - 2^(32 + shift) < Nq <= 2^(shift + 1) keeps the quotient exact below 2^31
+    a.shift = 0;
+    while ((2ll << a.shift) < s->Nq) ++a.shift;
+    a.mul = s->Nq == 1 ? 0 : (unsigned)(((1ull << (32 + a.shift)) + s->Nq - 1) / (unsigned)s->Nq);
     a.sq = at_stride(s->q_stride); a.sk = at_stride(s->k_stride); a.sv = at_stride(s->v_stride); a.so = at_stride(s->o_stride);
     a.sdo = at_stride(s->do_stride); a.sdq = at_stride(s->dq_stride); a.sdk = at_stride(s->dk_stride); a.sdv = at_stride(s->dv_stride);
 }
