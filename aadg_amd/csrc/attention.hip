@@ -503,9 +503,15 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
         }
 }
 
+// order of the key tiles: the ones most rows see (causal: the first) are dealt first, and the second half backwards, so that the two workgroups a
+// CU holds, number i and i + 256 of 512, are a long and a short one
+__device__ __forceinline__ int at_key_tile(const AtArgs& a, int rank) {
+    const int half = (a.tiles + 1) / 2;
+    return !a.causal || rank < half ? rank : a.tiles - 1 - (rank - half);
+}
+
 // dk, dv: a wave owns 32 keys (its K and V fragments stay in registers) and walks the folded rows, BQ at a time through LDS;
-// dv^T += dO^T P, dk^T += Q^T dS.  -D_i is the initial value of the dP accumulators.  Head widths over 64 in bfloat16 keep V in LDS (32 KB) to stay
-// within 256 registers, two waves per SIMD: with one the walk is a chain of waits (MFMA busy 19 %).
+// dv^T += dO^T P, dk^T += Q^T dS.  -D_i is the initial value of the dP accumulators.  (Head widths up to 64.)
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(const AtArgs a) {
     typedef At<T> M;
@@ -514,28 +520,23 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
     constexpr int LD = (BQ * CPR + NT - 1) / NT, DT = D / 32, PG = 16 / (KS / 2);
     __shared__ __attribute__((aligned(16))) T Qs[BQ * L_::PITCH];
     __shared__ __attribute__((aligned(16))) T Gs[BQ * L_::PITCH];
-    constexpr bool VL = false;
-    __shared__ __attribute__((aligned(16))) T Vs[VL ? 32 * NW * L_::PITCH : 8];
     __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
     __shared__ __attribute__((aligned(16))) int Es[BQ];                       // key limit of each row
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int sp = SPLIT ? blockIdx.x % a.splits : 0;
-    const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
-    const int bg = w / a.tiles, tile = w - bg * a.tiles, b = bg / a.G, g = bg - b * a.G;
+    const int n = a.B * a.G * (SPLIT ? a.splits : 1), rank = blockIdx.x / n, w = blockIdx.x - rank * n;
+    const int sp = SPLIT ? w % a.splits : 0, bg = SPLIT ? w / a.splits : w, tile = at_key_tile(a, rank), b = bg / a.G, g = bg - b * a.G;
     const int L = at_len(a, b);
     const int wg_key0 = tile * 32 * NW, key0 = wg_key0 + 32 * wv, key = key0 + (lane & 31);
     const T* kb = (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
     const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
     const float c = a.scale * AT_LOG2E;
     const int r_lo = SPLIT ? sp * a.chunk : 0, r_hi = wg_key0 < L ? (SPLIT ? min(a.R, r_lo + a.chunk) : a.R) : r_lo;      // (no key: nothing to walk)
-    typename M::Frag kf[U], vf[VL ? 1 : U];
+    typename M::Frag kf[U], vf[U];
     if (wg_key0 < L) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             kf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(kb, a.sk.n, key, L, 2 * u + h, a.d));
-            const at_u32x4 x = at_load<T>(vb, a.sv.n, key, L, 2 * u + h, a.d);
-            if (VL) *reinterpret_cast<at_u32x4*>(&Vs[L_::at(32 * wv + (lane & 31), 2 * u + h)]) = x;      // (read by this wave only)
-            else vf[u] = __builtin_bit_cast(typename M::Frag, x);
+            vf[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(vb, a.sv.n, key, L, 2 * u + h, a.d));
         }
     }
     f32x16 ak[DT], av[DT];
@@ -600,7 +601,7 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 s = M::mma(L_::rows(Qs, 32 * t, u, lane), kf[u], s);
-                dp = M::mma(L_::rows(Gs, 32 * t, u, lane), VL ? L_::rows(Vs, 32 * wv, u, lane) : vf[VL ? 0 : u], dp);
+                dp = M::mma(L_::rows(Gs, 32 * t, u, lane), vf[u], dp);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -659,6 +660,164 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
         }
 }
 
+// dk, dv for head widths over 64: a PAIR of waves owns 32 keys and walks the folded rows, BQ at a time through LDS.  Wave 0 of a pair keeps the keys' K fragments, takes
+// S = Q K^T, makes P and hands it over through LDS (lane to lane, float32), then accumulates dv^T += dO^T P; wave 1 keeps V, takes dP = dO V^T - D
+// (-D_i is the initial value of its accumulators), makes dS = P dP and accumulates dk^T += Q^T dS.  Both halves are the same code on swapped
+// operands and the same number of products; one wave doing both needs 2 D accumulator and D fragment registers and leaves a SIMD one
+// wave (D = 128: 423 us instead of XXX us for two sequences of 4096, 8 heads).
+template <typename T, int D, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
+    typedef At<T> M;
+    typedef Tile<T, D> L_;
+    constexpr int RT = sizeof(T) == 4 || NW == 2 ? 1 : 2, BQ = 32 * RT, NP = NW / 2, KS = M::KS, CH = M::CH, U = D / KS, CPR = D / CH, NT = 64 * NW;
+    constexpr int LD = (BQ * CPR + NT - 1) / NT, DT = D / 32, PG = 16 / (KS / 2);
+    __shared__ __attribute__((aligned(16))) T Xs[2 * BQ * L_::PITCH];         // Q, dO
+    __shared__ __attribute__((aligned(16))) float Ps[RT * NP * 1024];
+    __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
+    __shared__ __attribute__((aligned(16))) int Es[BQ];                       // key limit of each row
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, pair = wv >> 1, role = wv & 1;
+    const int n = a.B * a.G * (SPLIT ? a.splits : 1), rank = blockIdx.x / n, w = blockIdx.x - rank * n;
+    const int sp = SPLIT ? w % a.splits : 0, bg = SPLIT ? w / a.splits : w, tile = at_key_tile(a, rank), b = bg / a.G, g = bg - b * a.G;
+    const int L = at_len(a, b);
+    const int wg_key0 = tile * 32 * NP, key0 = wg_key0 + 32 * pair, key = key0 + (lane & 31);
+    const float c = a.scale * AT_LOG2E;
+    const int r_lo = SPLIT ? sp * a.chunk : 0, r_hi = wg_key0 < L ? (SPLIT ? min(a.R, r_lo + a.chunk) : a.R) : r_lo;      // (no key: nothing to walk)
+    typename M::Frag f[U];
+    if (wg_key0 < L) {
+        const T* base = role ? (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h : (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
+        const long long step = role ? a.sv.n : a.sk.n;
+#pragma unroll
+        for (int u = 0; u < U; ++u) f[u] = __builtin_bit_cast(typename M::Frag, at_load<T>(base, step, key, L, 2 * u + h, a.d));
+    }
+    f32x16 acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    // first tile from q0 on with a row that sees a key of this workgroup
+    auto next = [&](int q0) {
+        if (a.causal)
+            while (q0 < r_hi && at_limit_max(a, L, q0, BQ) <= wg_key0) q0 += BQ;
+        return q0;
+    };
+    at_u32x4 rq[LD], rg[LD];
+    float r_lse = 0.0f, r_d = 0.0f;
+    auto fetch = [&](int q0) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR, rr = min(q0 + rw, r_hi - 1);
+            rq[i] = at_fetch<T>((const T*)a.q + at_row(a, a.sq, b, g, rr), 0, 0, 1, ch, a.d);
+            rg[i] = at_fetch<T>((const T*)a.dout + at_row(a, a.sdo, b, g, rr), 0, 0, 1, ch, a.d);
+        }
+        const long long e = ((long long)b * a.G + g) * a.R + min(q0 + (tid & (BQ - 1)), r_hi - 1);
+        r_lse = a.lse[e];
+        r_d = a.delta[e];
+    };
+    const T *X1 = Xs + role * BQ * L_::PITCH, *X2 = Xs + (1 - role) * BQ * L_::PITCH;
+    aadg_f32x4* P = reinterpret_cast<aadg_f32x4*>(Ps) + pair * 256 + lane;
+    // a row that does not exist has lse = inf, i.e. p = 0: only the rows' limits can cut this pair's keys
+    const bool edge = a.causal || key0 + 32 > L;
+    int q0 = next(r_lo);
+    if (q0 < r_hi) fetch(q0);
+    while (q0 < r_hi) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
+            if (BQ * CPR % NT != 0 && id >= BQ * CPR) break;
+            const bool ok = q0 + rw < r_hi && ch * CH < a.d;
+            *reinterpret_cast<at_u32x4*>(&Xs[L_::at(rw, ch)]) = at_keep(rq[i], ok);
+            *reinterpret_cast<at_u32x4*>(&Xs[BQ * L_::PITCH + L_::at(rw, ch)]) = at_keep(rg[i], ok);
+        }
+        if (tid < BQ) {
+            const bool ok = q0 + tid < r_hi;
+            Ls[tid] = ok ? r_lse : INFINITY;
+            Ds[tid] = ok ? -r_d : 0.0f;
+            Es[tid] = ok ? at_limit(a, L, q0 + tid) : 0;
+        }
+        __syncthreads();
+        const int qn = next(q0 + BQ);
+        if (qn < r_hi) fetch(qn);
+        f32x16 s[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            if (role) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const aadg_f32x4 x = *reinterpret_cast<const aadg_f32x4*>(&Ds[32 * t + 8 * i + 4 * h]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][4 * i + e] = x[e];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) s[t] = M::mma(L_::rows(X1, 32 * t, u, lane), f[u], s[t]);
+        if (!role) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const aadg_f32x4 x = *reinterpret_cast<const aadg_f32x4*>(&Ls[32 * t + 8 * i + 4 * h]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][4 * i + e] = at_exp2(fmaf(s[t][4 * i + e], c, -x[e]));
+                }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int4 x = *reinterpret_cast<const int4*>(&Es[32 * t + 8 * i + 4 * h]);
+                        const int lim[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[t][4 * i + e] = key < lim[e] ? s[t][4 * i + e] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) P[1024 / 4 * NP * t + 64 * i] = aadg_f32x4{s[t][4 * i], s[t][4 * i + 1], s[t][4 * i + 2], s[t][4 * i + 3]};
+            }
+        }
+        __syncthreads();
+        if (role) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const aadg_f32x4 x = P[1024 / 4 * NP * t + 64 * i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][4 * i + e] *= x[e];
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int p = 0; p < PG; ++p) {
+                const typename M::Frag pf = M::pack(s[t], p);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) acc[dt] = M::mma(L_::cols(X2, 32 * t + KS * p, 32 * dt, lane), pf, acc[dt]);
+            }
+        q0 = qn;
+    }
+    if (key >= a.Nk) return;
+    const float sc = role ? a.scale : 1.0f;
+    const long long rows = (long long)a.B * a.G * a.Nk, flat = ((long long)b * a.G + g) * a.Nk + key;
+    T* out = role ? (T*)a.dk + b * a.sdk.b + (long long)g * a.sdk.h + (long long)key * a.sdk.n
+                  : (T*)a.dv + b * a.sdv.b + (long long)g * a.sdv.h + (long long)key * a.sdv.n;
+    float* part = SPLIT ? a.part + (2 * sp * rows + flat + (role ? 0 : rows)) * a.d : nullptr;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = 32 * t + 8 * i + 4 * h;
+            if (col >= a.d) continue;
+            const float4 x = make_float4(acc[t][4 * i] * sc, acc[t][4 * i + 1] * sc, acc[t][4 * i + 2] * sc, acc[t][4 * i + 3] * sc);
+            if (SPLIT) *reinterpret_cast<float4*>(part + col) = x;
+            else M::store4(out + col, x.x, x.y, x.z, x.w);
+        }
+}
+
 // sum of the splits' partials in split order, one lane per 4 values: out[b, head, n] = sum_s part[s * step + (b heads + head) n_rows + n];
 // a second row of workgroups takes a second tensor, whose partials lie behind the first's
 template <typename T>
@@ -710,9 +869,9 @@ struct AtPlan { int nw, tiles, splits, chunk; };
 // CU.  The join is a launch of its own (4 us), so a split keeps what takes as long: 256 / D tiles in bfloat16 (1 us a tile at D = 64), two at
 // D = 32 and one otherwise in float32 (5 us at D = 64); two where nearly nothing else runs (under a wave per four CUs) and a tile takes a
 // trip to memory, not its products.
-AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile) {
+AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile, int small) {
     AtPlan p;
-    p.nw = own <= 32 ? 1 : 4;
+    p.nw = own <= 32 * small ? small : 4;
     p.tiles = (own + 32 * p.nw - 1) / (32 * p.nw);
     const int64_t waves = (int64_t)s->B * s->G * p.tiles * p.nw;
     const int D = s->d <= 32 ? 32 : s->d <= 64 ? 64 : 128, work = s->dtype == 1 ? 256 / D : D == 32 ? 2 : 1;
@@ -726,8 +885,12 @@ AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile) {
     p.splits = (n + per - 1) / per;
     return p;
 }
-AtPlan at_plan_rows(const aadg_attention_desc* s) { return at_plan(s, s->H / s->G * s->Nq, s->Nk, 64); }
-AtPlan at_plan_keys(const aadg_attention_desc* s) { return at_plan(s, s->Nk, s->H / s->G * s->Nq, 32); }
+AtPlan at_plan_rows(const aadg_attention_desc* s) { return at_plan(s, s->H / s->G * s->Nq, s->Nk, 64, 1); }
+// (head widths over 64: a pair of waves has the 32 keys of a wave, so twice the keys are counted)
+AtPlan at_plan_keys(const aadg_attention_desc* s) {
+    const int f = s->d > 64 ? 2 : 1;
+    return at_plan(s, f * s->Nk, s->H / s->G * s->Nq, 32, f);
+}
 
 size_t at_fwd_bytes(const aadg_attention_desc* s) {
     const AtPlan p = at_plan_rows(s);
@@ -753,21 +916,21 @@ void at_use(AtArgs& a, const AtPlan& p) { a.tiles = p.tiles; a.splits = p.splits
         if (p.splits > 1) hipLaunchKernelGGL((KERNEL<T, D, NW, true>), grid, dim3(64 * NW), 0, st, a);                     \
         else hipLaunchKernelGGL((KERNEL<T, D, NW, false>), grid, dim3(64 * NW), 0, st, a);                                 \
     } while (0)
-#define AT_BY_NW(KERNEL, T, D)                                                                                             \
+#define AT_BY_NW(KERNEL, T, D, SMALL)                                                                                      \
     do {                                                                                                                   \
-        if (p.nw == 1) AT_LAUNCH(KERNEL, T, D, 1);                                                                         \
-        else AT_LAUNCH(KERNEL, T, D, 4);                                                                                   \
+        if (p.nw == 4) AT_LAUNCH(KERNEL, T, D, 4);                                                                         \
+        else AT_LAUNCH(KERNEL, T, D, SMALL);                                                                               \
     } while (0)
-#define AT_BY_D(KERNEL, T)                                                                                                 \
+#define AT_BY_D(KERNEL, T, WIDE, SMALL)                                                                                    \
     do {                                                                                                                   \
-        if (a.d <= 32) AT_BY_NW(KERNEL, T, 32);                                                                            \
-        else if (a.d <= 64) AT_BY_NW(KERNEL, T, 64);                                                                       \
-        else AT_BY_NW(KERNEL, T, 128);                                                                                     \
+        if (a.d <= 32) AT_BY_NW(KERNEL, T, 32, 1);                                                                         \
+        else if (a.d <= 64) AT_BY_NW(KERNEL, T, 64, 1);                                                                    \
+        else AT_BY_NW(WIDE, T, 128, SMALL);                                                                                \
     } while (0)
 
 template <typename T> int at_forward(AtArgs& a, const AtPlan& p, hipStream_t st) {
     at_use(a, p);
-    AT_BY_D(k_attn_fwd, T);
+    AT_BY_D(k_attn_fwd, T, k_attn_fwd, 1);
     AADG_LAUNCH_CHECK();
     if (p.splits > 1) {
         const long long n = (long long)a.B * a.H * a.Nq;
@@ -782,7 +945,7 @@ template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, h
     if (a.dq != nullptr) {
         const AtPlan p = at_plan_rows(s);
         at_use(a, p);
-        AT_BY_D(k_attn_dq, T);                                                // leaves D_i in a.delta
+        AT_BY_D(k_attn_dq, T, k_attn_dq, 1);                                                // leaves D_i in a.delta
         AADG_LAUNCH_CHECK();
         if (p.splits > 1) {
             const long long n = rows * (a.d / 4);
@@ -797,7 +960,7 @@ template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, h
     if (a.dk != nullptr) {
         const AtPlan p = at_plan_keys(s);
         at_use(a, p);
-        AT_BY_D(k_attn_dkv, T);
+        AT_BY_D(k_attn_dkv, T, k_attn_dkv_pair, 2);
         AADG_LAUNCH_CHECK();
         if (p.splits > 1) {
             const long long nk = (long long)a.B * a.G * a.Nk, n = nk * (a.d / 4);
