@@ -818,6 +818,184 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
         }
 }
 
+// The whole backward in one walk over the rows, where a workgroup can hold every key (bfloat16, head widths 33 ... 64, at most 32 NW keys): five
+// products instead of seven, and q, o, dO are read once.  Wave w owns keys 32 w ... + 31 as in k_attn_dkv; dS^T of all waves meets in LDS
+// ([key][row], 72 bytes a key: 8-byte writes of neighbouring keys and the transpose reads spread over the banks), and dq^T = K^T dS^T is taken in
+// 16 x 16 tiles (v_mfma_f32_16x16x32_bf16: every wave has its tiles over all keys, no sum across waves; its K^T fragments stay in registers).
+// D_i comes from the rows on their way to LDS (eight neighbouring lanes hold a row).
+template <int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_bwd_short(const AtArgs a) {
+    typedef uint16_t T;
+    typedef At<T> M;
+    constexpr int D = 64, BQ = 32, KS = 16, U = D / KS, DT = D / 32, NS = NW, RH = NW == 8 ? 1 : 2, SP = 36;      // NS: 32-key steps; RH: row halves per wave; SP: dS^T pitch
+    typedef Tile<T, D> L_;
+    __shared__ __attribute__((aligned(16))) T Qs[BQ * L_::PITCH];
+    __shared__ __attribute__((aligned(16))) T Gs[BQ * L_::PITCH];
+    __shared__ __attribute__((aligned(16))) T Ss[32 * NW * SP];
+    __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
+    __shared__ __attribute__((aligned(16))) int Es[BQ];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int sp = SPLIT ? blockIdx.x % a.splits : 0, bg = SPLIT ? blockIdx.x / a.splits : blockIdx.x, b = bg / a.G, g = bg - b * a.G;
+    const int L = at_len(a, b), Lc = max(L, 1);                               // (a sequence without keys reads key 0, masked)
+    const int key0 = 32 * wv, key = key0 + (lane & 31);
+    const T* kb = (const T*)a.k + b * a.sk.b + (long long)g * a.sk.h;
+    const T* vb = (const T*)a.v + b * a.sv.b + (long long)g * a.sv.h;
+    const float c = a.scale * AT_LOG2E;
+    const int r_lo = SPLIT ? sp * a.chunk : 0, r_hi = SPLIT ? min(a.R, r_lo + a.chunk) : a.R;
+    typename M::Frag kf[U], vf[U], kt[NS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const bool ok = key < L && (2 * u + h) * 8 < a.d;
+        kf[u] = __builtin_bit_cast(typename M::Frag, at_keep(at_fetch<T>(kb, a.sk.n, key, Lc, 2 * u + h, a.d), ok));
+        vf[u] = __builtin_bit_cast(typename M::Frag, at_keep(at_fetch<T>(vb, a.sv.n, key, Lc, 2 * u + h, a.d), ok));
+    }
+    // K^T fragments of this wave's 16 columns: lane & 15 = column, eight keys per 16 lanes in the order the dS^T reads give: 8 (lane >> 4) + 0 ... 7
+    const int dq0 = 16 * (wv & 3), rh0 = NW == 8 ? wv >> 2 : 0, kcol = dq0 + (lane & 15);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        uint32_t x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int kk = 32 * n + 8 * (lane >> 4) + e;
+            const T val = kb[(long long)min(kk, Lc - 1) * a.sk.n + min(kcol, a.d - 1)];
+            x[e] = kk < L && kcol < a.d ? val : 0;
+        }
+        const at_u32x4 y = {x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16};
+        kt[n] = __builtin_bit_cast(typename M::Frag, y);
+    }
+    f32x16 ak[DT], av[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ak[t][i] = av[t][i] = 0.0f;
+    // 256 chunks of each of q, dO, o per tile: eight waves split them (q | dO and o), four take all
+    const bool has_q = NW == 4 || tid < 256, has_g = NW == 4 || tid >= 256;
+    const int rw = (tid & 255) >> 3, ch = tid & 7;
+    at_u32x4 rq = {}, rg = {}, ro = {};
+    float r_lse = 0.0f;
+    auto fetch = [&](int q0) {
+        const int rr = min(q0 + rw, r_hi - 1);
+        if (has_q) rq = at_fetch<T>((const T*)a.q + at_row(a, a.sq, b, g, rr), 0, 0, 1, ch, a.d);
+        if (has_g) {
+            rg = at_fetch<T>((const T*)a.dout + at_row(a, a.sdo, b, g, rr), 0, 0, 1, ch, a.d);
+            ro = at_fetch<T>((const T*)a.o + at_row(a, a.so, b, g, rr), 0, 0, 1, ch, a.d);
+        }
+        r_lse = a.lse[((long long)b * a.G + g) * a.R + min(q0 + (tid & 31), r_hi - 1)];
+    };
+    const bool edge = a.causal || key0 + 32 > L;
+    fetch(r_lo);
+    for (int q0 = r_lo; q0 < r_hi; q0 += BQ) {
+        // (the last reads of Qs, Gs lie before the barrier in the middle of the last tile, those of Ss before the next barrier)
+        const bool ok = q0 + rw < r_hi && ch * 8 < a.d;
+        if (has_q) *reinterpret_cast<at_u32x4*>(&Qs[L_::at(rw, ch)]) = at_keep(rq, ok);
+        if (has_g) {
+            const at_u32x4 x = at_keep(rg, ok);
+            *reinterpret_cast<at_u32x4*>(&Gs[L_::at(rw, ch)]) = x;
+            float dl = M::dot(__builtin_bit_cast(typename M::Frag, x), __builtin_bit_cast(typename M::Frag, at_keep(ro, ok)), 0.0f);
+            dl += __shfl_xor(dl, 1, 64);
+            dl += __shfl_xor(dl, 2, 64);
+            dl += __shfl_xor(dl, 4, 64);
+            if (ch == 0) Ds[rw] = -dl;
+        }
+        if (tid < BQ) {
+            const bool live = q0 + tid < r_hi;
+            Ls[tid] = live ? r_lse : INFINITY;
+            Es[tid] = live ? at_limit(a, L, q0 + tid) : 0;
+        }
+        __syncthreads();
+        if (q0 + BQ < r_hi) fetch(q0 + BQ);
+        f32x16 s, dp;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const aadg_f32x4 x = *reinterpret_cast<const aadg_f32x4*>(&Ds[8 * i + 4 * h]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[4 * i + e] = 0.0f;
+                dp[4 * i + e] = x[e];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s = M::mma(L_::rows(Qs, 0, u, lane), kf[u], s);
+            dp = M::mma(L_::rows(Gs, 0, u, lane), vf[u], dp);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const aadg_f32x4 x = *reinterpret_cast<const aadg_f32x4*>(&Ls[8 * i + 4 * h]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * i + e] = at_exp2(fmaf(s[4 * i + e], c, -x[e]));
+        }
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int4 x = *reinterpret_cast<const int4*>(&Es[8 * i + 4 * h]);
+                const int lim[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[4 * i + e] = key < lim[e] ? s[4 * i + e] : 0.0f;
+                    dp[4 * i + e] = key < lim[e] ? dp[4 * i + e] : 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const typename M::Frag pf = M::pack(s, p), df = M::pack(dp, p);
+            const at_u32x4 dw = __builtin_bit_cast(at_u32x4, df);             // rows 16 p + 4 h + 0 ... 3 and + 8
+            *reinterpret_cast<uint2*>(&Ss[key * SP + 16 * p + 4 * h]) = make_uint2(dw[0], dw[1]);
+            *reinterpret_cast<uint2*>(&Ss[key * SP + 16 * p + 8 + 4 * h]) = make_uint2(dw[2], dw[3]);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                av[dt] = M::mma(L_::cols(Gs, KS * p, 32 * dt, lane), pf, av[dt]);
+                ak[dt] = M::mma(L_::cols(Qs, KS * p, 32 * dt, lane), df, ak[dt]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+            const int rr0 = 16 * (rh0 + r);
+            aadg_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                // B operand: lane & 15 = row, keys 32 n + 8 (lane >> 4) + 0 ... 7 (lane i of 16 passes key i / 4, rows 4 (i % 4), and gets 4 keys of row i)
+                const T* q = &Ss[(32 * n + 8 * (lane >> 4) + ((lane & 15) >> 2)) * SP + rr0 + 4 * (lane & 3)];
+                typedef at_v4i16 __attribute__((address_space(3)))* lds_p;
+                const at_v4i16 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(q)), v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(q + 4 * SP));
+                typedef short v8i16 __attribute__((ext_vector_type(8)));
+                const v8i16 v = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kt[n], __builtin_bit_cast(at_bf16x8, v), y, 0, 0, 0);
+            }
+            const int row = q0 + rr0 + (lane & 15), col = dq0 + 4 * (lane >> 4);      // C: lane & 15 = row, register e = column 4 (lane >> 4) + e
+            if (row < r_hi && col < a.d)
+                M::store4((T*)a.dq + at_row(a, a.sdq, b, g, row) + col, y[0] * a.scale, y[1] * a.scale, y[2] * a.scale, y[3] * a.scale);
+        }
+    }
+    if (key >= a.Nk) return;
+    const float sc = a.scale;
+    const long long rows = (long long)a.B * a.G * a.Nk, flat = ((long long)b * a.G + g) * a.Nk + key;
+    T* kp = (T*)a.dk + b * a.sdk.b + (long long)g * a.sdk.h + (long long)key * a.sdk.n;
+    T* vp = (T*)a.dv + b * a.sdv.b + (long long)g * a.sdv.h + (long long)key * a.sdv.n;
+    float* pk = SPLIT ? a.part + (2 * sp * rows + flat) * a.d : nullptr;
+    float* pv = SPLIT ? pk + rows * a.d : nullptr;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = 32 * t + 8 * i + 4 * h;
+            if (col >= a.d) continue;
+            const float4 x = make_float4(ak[t][4 * i] * sc, ak[t][4 * i + 1] * sc, ak[t][4 * i + 2] * sc, ak[t][4 * i + 3] * sc);
+            const float4 y = make_float4(av[t][4 * i], av[t][4 * i + 1], av[t][4 * i + 2], av[t][4 * i + 3]);
+            if (SPLIT) {
+                *reinterpret_cast<float4*>(pk + col) = x;
+                *reinterpret_cast<float4*>(pv + col) = y;
+            } else {
+                M::store4(kp + col, x.x, x.y, x.z, x.w);
+                M::store4(vp + col, y.x, y.y, y.z, y.w);
+            }
+        }
+}
+
 // sum of the splits' partials in split order, one lane per 4 values: out[b, head, n] = sum_s part[s * step + (b heads + head) n_rows + n];
 // a second row of workgroups takes a second tensor, whose partials lie behind the first's
 template <typename T>
@@ -892,6 +1070,27 @@ AtPlan at_plan_keys(const aadg_attention_desc* s) {
     return at_plan(s, f * s->Nk, s->H / s->G * s->Nq, 32, f);
 }
 
+// The one-walk backward: keys a workgroup can hold.  Splits of the rows by what they cost: a tile of 32 rows takes 2 us, the workgroups (one of eight
+// waves or two of four to a CU) run in rounds, and every split writes and reads its dk and dv in float32 (4 us for the join, 4.7 TB/s).
+bool at_is_short(const aadg_attention_desc* s) { return s->dtype == 1 && s->d > 32 && s->d <= 64 && s->Nk > 32 && s->Nk <= 256; }
+AtPlan at_plan_short(const aadg_attention_desc* s) {
+    AtPlan p;
+    p.nw = s->Nk <= 128 ? 4 : 8;
+    p.tiles = 1;
+    const int64_t R = (int64_t)(s->H / s->G) * s->Nq, bg = (int64_t)s->B * s->G, n = (R + 31) / 32, slots = p.nw == 4 ? 512 : 256;
+    const double join = 16.0 * bg * s->Nk * s->d / 4.7e6;
+    double best = 0.0;
+    for (int64_t sp = 1; sp <= 64 && sp <= n; ++sp) {
+        const int64_t len = (n + sp - 1) / sp;
+        const double cost = 2.0 * ((bg * sp + slots - 1) / slots) * len + (sp > 1 ? 4.0 + join * sp : 0.0);
+        if (sp > 1 && cost >= best) continue;
+        best = cost;
+        p.chunk = (int)(len * 32);
+        p.splits = (int)((n + len - 1) / len);
+    }
+    return p;
+}
+
 size_t at_fwd_bytes(const aadg_attention_desc* s) {
     const AtPlan p = at_plan_rows(s);
     return p.splits > 1 ? (size_t)p.splits * s->B * s->H * s->Nq * (s->d + 2) * 4 : 0;
@@ -940,8 +1139,30 @@ template <typename T> int at_forward(AtArgs& a, const AtPlan& p, hipStream_t st)
     return 0;
 }
 
+template <typename T> int at_sum_kv(const AtArgs& a, int splits, hipStream_t st) {
+    const long long nk = (long long)a.B * a.G * a.Nk, n = nk * (a.d / 4);
+    hipLaunchKernelGGL(k_attn_sum<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, st, a.part, (T*)a.dk, a.sdk, (T*)a.dv, a.sdv, a.B, a.G, a.Nk,
+                       a.d, splits, 2 * nk * a.d);
+    AADG_LAUNCH_CHECK();
+    return 0;
+}
+
 template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, hipStream_t st) {
     const long long rows = (long long)a.B * a.H * a.Nq;
+    if (a.dq != nullptr && a.dk != nullptr && at_is_short(s)) {
+        const AtPlan p = at_plan_short(s);
+        at_use(a, p);
+        const dim3 grid((unsigned)((long long)a.B * a.G * p.splits));
+        if (p.nw == 8) {
+            if (p.splits > 1) hipLaunchKernelGGL((k_attn_bwd_short<8, true>), grid, dim3(512), 0, st, a);
+            else hipLaunchKernelGGL((k_attn_bwd_short<8, false>), grid, dim3(512), 0, st, a);
+        } else {
+            if (p.splits > 1) hipLaunchKernelGGL((k_attn_bwd_short<4, true>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((k_attn_bwd_short<4, false>), grid, dim3(256), 0, st, a);
+        }
+        AADG_LAUNCH_CHECK();
+        return p.splits > 1 ? at_sum_kv<T>(a, p.splits, st) : 0;
+    }
     if (a.dq != nullptr) {
         const AtPlan p = at_plan_rows(s);
         at_use(a, p);
@@ -962,12 +1183,7 @@ template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, h
         at_use(a, p);
         AT_BY_D(k_attn_dkv, T, k_attn_dkv_pair, 2);
         AADG_LAUNCH_CHECK();
-        if (p.splits > 1) {
-            const long long nk = (long long)a.B * a.G * a.Nk, n = nk * (a.d / 4);
-            hipLaunchKernelGGL(k_attn_sum<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, st, a.part, (T*)a.dk, a.sdk, (T*)a.dv, a.sdv, a.B,
-                               a.G, a.Nk, a.d, p.splits, 2 * nk * a.d);
-            AADG_LAUNCH_CHECK();
-        }
+        if (p.splits > 1) return at_sum_kv<T>(a, p.splits, st);
     }
     return 0;
 }
@@ -984,9 +1200,10 @@ extern "C" size_t aadg_attention_forward_workspace_bytes(const aadg_attention_de
 
 extern "C" size_t aadg_attention_backward_workspace_bytes(const aadg_attention_desc* desc_host) {
     if (at_check(desc_host) != 0) return 0;
-    const AtPlan pk = at_plan_keys(desc_host), pq = at_plan_rows(desc_host);
+    const AtPlan pk = at_plan_keys(desc_host), pq = at_plan_rows(desc_host), ps = at_plan_short(desc_host);
     const size_t row = (size_t)desc_host->d * 4;
-    const size_t nk = pk.splits > 1 ? (size_t)pk.splits * 2 * desc_host->B * desc_host->G * desc_host->Nk * row : 0;
+    const int sk = at_is_short(desc_host) && ps.splits > pk.splits ? ps.splits : pk.splits;
+    const size_t nk = sk > 1 ? (size_t)sk * 2 * desc_host->B * desc_host->G * desc_host->Nk * row : 0;
     const size_t nq = pq.splits > 1 ? (size_t)pq.splits * desc_host->B * desc_host->H * desc_host->Nq * row : 0;
     return at_delta_bytes(desc_host) + (nk > nq ? nk : nq);          // dq is joined before dk / dv reuse the partials
 }

@@ -89,6 +89,13 @@ SHAPES = [
     (1, 2, 1, 2000, 40, 64, False, None),                   # many rows, few keys: split over the rows
     (1, 1, 1, 3, 3, 16, True, [2]),
     (1, 1, 1, 513, 700, 104, True, None),
+    # bfloat16, 33 ... 256 keys, widths 33 ... 64: every key in one workgroup
+    (2, 4, 2, 150, 200, 48, True, [200, 0]),
+    (1, 1, 1, 1100, 256, 64, False, None),
+    (2, 2, 1, 600, 100, 64, True, [100, 37]),
+    (3, 1, 1, 31, 33, 40, False, None),
+    (2, 2, 2, 1030, 250, 56, False, [250, 129]),
+    (300, 1, 1, 40, 129, 64, False, None),
 ]
 
 
