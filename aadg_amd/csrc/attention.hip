@@ -1026,11 +1026,12 @@ AtStride at_stride(const int64_t* s) { return AtStride{s[0], s[1], s[2]}; }
 // 0, or the error of a descriptor the kernels do not take.  16-byte rows: every stride and pointer a multiple of 16 bytes.
 int at_check(const aadg_attention_desc* s) {
     if (s == nullptr || s->dtype < 0 || s->dtype > 1 || s->B < 1 || s->H < 1 || s->G < 1 || s->Nq < 1 || s->Nk < 1 || s->d < 1) return AADG_E_BADARG;
-    if (!(s->scale > 0.0f) || !(s->scale < INFINITY)) return AADG_E_BADARG;
+    if (!(s->scale > 0.0f) || !(s->scale * AT_LOG2E < INFINITY)) return AADG_E_BADARG;
     if (s->H % s->G != 0) return AADG_E_BADARG;
     if (s->d % 8 != 0 || s->d > 128) return AADG_E_UNSUPPORTED;
     const int64_t r = s->H / s->G, R = r * s->Nq;
-    if (R > (1 << 30) || s->Nk > (1 << 30) || (int64_t)s->B * s->H > (1 << 20)) return AADG_E_UNSUPPORTED;
+    if (R > (1 << 29) || s->Nk > (1 << 29) || (int64_t)s->B * s->H > (1 << 20)) return AADG_E_UNSUPPORTED;
+    if ((int64_t)s->B * s->H * s->Nq / 4 >= 0x7FFFFFFF) return AADG_E_UNSUPPORTED;
     // grids: at most (rows or keys) / 32 tiles per group, 64 splits
     if ((int64_t)s->B * s->G * (((R > s->Nk ? R : s->Nk) + 31) / 32) * 64 > 0x7FFFFFFF) return AADG_E_UNSUPPORTED;
     if ((int64_t)s->B * s->H * s->Nq * (s->d / 4) / 256 >= 0x7FFFFFFF || (int64_t)s->B * s->G * s->Nk * (s->d / 4) / 256 >= 0x7FFFFFFF) return AADG_E_UNSUPPORTED;

@@ -74,18 +74,6 @@ __device__ __forceinline__ int or_find(const OrMat* __restrict__ table, int coun
     return __builtin_amdgcn_readfirstlane(at);
 }
 
-__device__ __forceinline__ void or_split(float x, uint16_t* p) {
-    const uint32_t h = aadg_f2bf_bits(x);
-    const float r = x - __uint_as_float(h << 16);
-    const uint32_t g = aadg_f2bf_bits(r);
-    p[0] = (uint16_t)h;
-    p[1] = (uint16_t)g;
-    p[2] = (uint16_t)aadg_f2bf_bits(r - __uint_as_float(g << 16));
-}
-__device__ __forceinline__ float or_join(uint16_t a, uint16_t b, uint16_t c) {
-    return __uint_as_float((uint32_t)a << 16) + (__uint_as_float((uint32_t)b << 16) + __uint_as_float((uint32_t)c << 16));
-}
-
 // partial sums of squares in double (squares of small gradients leave float32's range), OR_SUM elements a workgroup
 __global__ __launch_bounds__(256) void k_or_sum(const OrMat* __restrict__ table, int count, char* __restrict__ ws) {
     __shared__ double part[4];
@@ -93,53 +81,16 @@ __global__ __launch_bounds__(256) void k_or_sum(const OrMat* __restrict__ table,
     const int w = blockIdx.x - t.first[OR_P_SUM];
     const long long total = (long long)t.rows * t.cols, lo = (long long)w * OR_SUM, hi = min(total, lo + OR_SUM);
     double s = 0.0;
+    const float* src = t.src;
+#pragma unroll 8
     for (long long i = lo + threadIdx.x; i < hi; i += 256) {
-        const double x = t.src[i];
+        const double x = src[i];
         s = fma(x, x, s);
     }
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) reinterpret_cast<double*>(ws + t.sums)[w] = (part[0] + part[1]) + (part[2] + part[3]);
-}
-
-// X = U / (|U| + eps) as planes, 32 x 32 elements a workgroup, transposed through LDS where U is tall
-__global__ __launch_bounds__(256) void k_or_planes(const OrMat* __restrict__ table, int count, char* __restrict__ ws, float eps) {
-    __shared__ float tile[32][33];
-    __shared__ float scale_s;
-    const OrMat& t = table[or_find(table, count, OR_P_SPLIT, blockIdx.x)];
-    const int w = blockIdx.x - t.first[OR_P_SPLIT], tn = (t.ldx + 31) / 32;
-    const int r0 = w / tn * 32, c0 = (w - w / tn * tn) * 32;
-    if (threadIdx.x < 64) {
-        const int parts = (int)(((long long)t.rows * t.cols + OR_SUM - 1) / OR_SUM);
-        const double* p = reinterpret_cast<const double*>(ws + t.sums);
-        double s = 0.0;
-        for (int i = threadIdx.x; i < parts; i += 64) s += p[i];
-        s = wave_sum(s);
-        if (threadIdx.x == 0) scale_s = (float)(1.0 / (sqrt(s) + (double)eps));
-    }
-    const bool tall = t.rows > t.cols;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int y = ty + 8 * i;
-        // X[r0 + y][c0 + tx] = U[..][..]; tall: U[c0 + y][r0 + tx] = X[r0 + tx][c0 + y]
-        if (!tall) tile[y][tx] = r0 + y < t.m && c0 + tx < t.n ? t.src[(long long)(r0 + y) * t.cols + c0 + tx] : 0.0f;
-        else tile[tx][y] = c0 + y < t.n && r0 + tx < t.m ? t.src[(long long)(c0 + y) * t.cols + r0 + tx] : 0.0f;
-    }
-    __syncthreads();
-    const float scale = scale_s;
-    uint16_t* x = reinterpret_cast<uint16_t*>(ws + t.buf[OR_B_X0]);
-    const long long plane = (long long)t.m * t.ldx;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = r0 + ty + 8 * i, c = c0 + tx;
-        if (r >= t.m || c >= t.ldx) continue;
-        uint16_t p[3];
-        or_split(tile[ty + 8 * i][tx] * scale, p);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) x[k * plane + (long long)r * t.ldx + c] = p[k];
-    }
 }
 
 // LDS layouts.  K-contiguous operand: rows of BK values, the 16-byte chunks of a row permuted such that 8 rows of one chunk hit all banks.
@@ -182,6 +133,46 @@ __device__ __forceinline__ void or_load8(const uint16_t* p, long long plane, flo
     for (int i = 0; i < 4; ++i) {
         v[2 * i] = __uint_as_float(a[i] << 16) + (__uint_as_float(b[i] << 16) + __uint_as_float(c[i] << 16));
         v[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u) + (__uint_as_float(b[i] & 0xFFFF0000u) + __uint_as_float(c[i] & 0xFFFF0000u));
+    }
+}
+
+// X = U / (|U| + eps) as planes, 64 x 64 elements a workgroup, transposed through LDS where U is tall
+__global__ __launch_bounds__(256) void k_or_planes(const OrMat* __restrict__ table, int count, char* __restrict__ ws, float eps) {
+    __shared__ float tile[64][65];
+    __shared__ float scale_s;
+    const OrMat& t = table[or_find(table, count, OR_P_SPLIT, blockIdx.x)];
+    const int m = t.m, n = t.n, ldx = t.ldx, cols = t.cols, tn = ldx / 64;
+    const int w = blockIdx.x - t.first[OR_P_SPLIT], r0 = w / tn * 64, c0 = (w - w / tn * tn) * 64;
+    const float* src = t.src;
+    const bool tall = t.rows > t.cols;
+    if (threadIdx.x < 64) {
+        const int parts = (int)(((long long)t.rows * cols + OR_SUM - 1) / OR_SUM);
+        const double* p = reinterpret_cast<const double*>(ws + t.sums);
+        double s = 0.0;
+        for (int i = threadIdx.x; i < parts; i += 64) s += p[i];
+        s = wave_sum(s);
+        if (threadIdx.x == 0) scale_s = (float)(1.0 / (sqrt(s) + (double)eps));
+    }
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int y = ty + 4 * i;
+        // X[r0 + y][c0 + tx]; tall: U[c0 + y][r0 + tx] = X[r0 + tx][c0 + y]
+        if (!tall) tile[y][tx] = r0 + y < m && c0 + tx < n ? src[(long long)min(r0 + y, m - 1) * cols + min(c0 + tx, n - 1)] : 0.0f;
+        else tile[tx][y] = c0 + y < n && r0 + tx < m ? src[(long long)min(c0 + y, n - 1) * cols + min(r0 + tx, m - 1)] : 0.0f;
+    }
+    __syncthreads();
+    const float scale = scale_s;
+    uint16_t* x = reinterpret_cast<uint16_t*>(ws + t.buf[OR_B_X0]);
+    const long long plane = (long long)m * ldx;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = (threadIdx.x >> 3) + 32 * i, c = (threadIdx.x & 7) * 8;
+        if (r0 + r >= m) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e] * scale;
+        or_store8(x + (long long)(r0 + r) * ldx + c0 + c, plane, v);
     }
 }
 
@@ -513,7 +504,7 @@ int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out, const i
         for (int b = 0; b < OR_BUFS; ++b) { t.buf[b] = (long long)at; at += b == OR_B_X0 || b == OR_B_X1 ? px : pa; }
         t.sums = (long long)at; at += aadg_align_up((size_t)parts * 8, 256);
         t.part = (long long)at; at += t.splits > 1 ? (size_t)ts * t.splits * lay.tb_sym * lay.tb_sym * 4 : 0;
-        const long long wgs[OR_PHASES] = {parts, (long long)((t.m + 31) / 32) * ((t.ldx + 31) / 32), ts * t.splits, ts, xm * xn};
+        const long long wgs[OR_PHASES] = {parts, (long long)((t.m + 63) / 64) * (t.ldx / 64), ts * t.splits, ts, xm * xn};
         for (int p = 0; p < OR_PHASES; ++p) {
             t.first[p] = (int)lay.grid[p];
             lay.grid[p] += wgs[p];

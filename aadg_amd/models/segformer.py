@@ -15,8 +15,9 @@ SegFormer checkpoint's state_dict maps onto it.
 MI355X-first choices (same function, different schedule):
   * tokens stay [B, N, C] and bfloat16 through a stage (the Linear layers are plain hipBLASLt GEMMs on them); every residual add
     is folded into the LayerNorm that follows it (csrc/layernorm.hip: add + stochastic-depth factor + normalise in one pass, in the
-    tokens' own dtype -- no float32 residual stream, no casts around the norms); attention is
-    `scaled_dot_product_attention`; the Mix-FFN's depthwise convolution reads the same buffer through a channels-last view;
+    tokens' own dtype -- no float32 residual stream, no casts around the norms); attention reads the projections' outputs in place
+    and recomputes its probabilities in the backward (csrc/attention.hip); the Mix-FFN's depthwise convolution reads the same
+    buffer through a channels-last view;
   * the head never builds the 4 x 768-channel concatenation at stride 4 (14.5 GB in bf16 for 144 images of 512x512):
     a 1x1 convolution commutes with bilinear interpolation, so the fuse convolution's slice for stage i is folded into that
     stage's Linear (one [768, C_i] matrix, rebuilt from the reference-layout parameters each step), applied at the stage's own

@@ -233,6 +233,21 @@ def test_empty_inputs(hip):
     assert o.shape == q2.shape and not o.any() and not torch.autograd.grad(o.sum(), q2)[0].any()
 
 
+def test_offsets_past_32_bits(hip):
+    """rows 2^24 elements apart: the last of 200 lies 6.7 GB into the buffer"""
+    n, d = 200, 64
+    buf = torch.empty(n << 24, dtype=torch.bfloat16, device="cuda")
+    q, k, v, do = inputs(torch.bfloat16, 1, 1, 1, 40, n, d, seed=2)
+    far = [buf[64 * i:].as_strided((1, 1, n, d), (0, 0, 1 << 24, 1)) for i in range(2)]
+    far[0].copy_(k)
+    far[1].copy_(v)
+    got = hip.attention(q, *far)
+    assert torch.equal(got, hip.attention(q, k, v))
+    leaves, near = [t.detach().requires_grad_(True) for t in far], [t.clone().requires_grad_(True) for t in (k, v)]
+    for a, b in zip(torch.autograd.grad(hip.attention(q, *leaves), leaves, do), torch.autograd.grad(hip.attention(q, *near), near, do)):
+        assert torch.equal(a, b)
+
+
 def test_other_stream_and_captured_graph(hip):
     """A captured forward + backward replays on new inputs to the eager bits; two graphs and eager work keep apart."""
     shape = (2, 2, 1, 40, 1200, 64)

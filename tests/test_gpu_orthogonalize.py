@@ -94,6 +94,22 @@ def test_strided_and_unaligned(hip):
     assert torch.equal(hip.orthogonalize([v])[0], hip.orthogonalize([u])[0])
 
 
+def test_in_place_through_the_library(hip):
+    """aadg_orthogonalize_f32 with dst == src (aadg_hip.h allows it), and the same matrix twice in a list"""
+    import ctypes
+    u, v = matrix(70, 130), matrix(90, 20)
+    want = hip.orthogonalize([u, v, u])
+    assert torch.equal(want[0], want[2])
+    a, b = u.clone(), v.clone()
+    arr = (hip._Matrix * 2)((a.data_ptr(), a.data_ptr(), 70, 130), (b.data_ptr(), b.data_ptr(), 90, 20))
+    lib = hip.load()
+    need = lib.aadg_orthogonalize_workspace_bytes(arr, 2)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    f = ctypes.c_float
+    assert lib.aadg_orthogonalize_f32(arr, 2, 5, f(COEF[0]), f(COEF[1]), f(COEF[2]), f(1e-7), ws.data_ptr(), need, hip._stream()) == 0
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
 def test_stream_and_graph(hip):
     mats = [matrix(64, 200), matrix(300, 40), matrix(128, 128)]
     want = hip.orthogonalize(mats)
