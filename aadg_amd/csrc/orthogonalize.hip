@@ -1,9 +1,10 @@
 // Orthogonalised updates: a list of float32 matrices U is replaced by an odd polynomial of each that moves its singular values towards
 // one (Newton-Schulz iteration with the quintic the Muon optimiser uses), for the trained matrices of the segmentation networks.
 //
-//   X = U / (|U|_F + eps);   steps times:   A = X X^T,   B = b A + c A A,   X <- a X + B X          (X [m, n], m <= n: U or U^T)
+//   X = U / (|U|_F + eps);   steps times:   A = X X^T,   X <- P X,   P = a I + b A + c A A           (X [m, n], m <= n: U or U^T)
 //
-// Flops per step: m^2 n + m^3 (two symmetric products, one triangle each) + 2 m^2 n.
+// Flops per step: m^2 n + m^3 (two symmetric products, one triangle each) + 2 m^2 n.  The next step's A is P A P, symmetric as well, so several
+// steps can stay on [m, m] matrices before their product is applied to X: done for wide matrices (or_group).
 // The iteration magnifies small singular values by a per step, and with them whatever error the products leave (bfloat16 products: 1e-2 of
 // the result after five steps, products of two bfloat16 halves 4e-5, float32 3e-6), so the products are float32-grade: every operand
 // is kept as THREE bfloat16 planes, x = x0 + x1 + x2 (24 significant bits), and a product is the six plane products of weight 2^-16 or
@@ -447,46 +448,65 @@ __global__ __launch_bounds__(OR_NT) void k_or_reduce(const OrMat* __restrict__ t
 // ------------------------------------------------------------------------------------------------ host
 constexpr int OR_MAX_SIDE = 1 << 16, OR_MAX_MATS = 4096;
 
-struct OrLayout { size_t bytes; long long grid[OR_PHASES]; int tb_sym, tb_x; bool split; };
+struct OrLayout { size_t bytes; long long grid[OR_PHASES]; int n, tb_sym, tb_x; bool split; };
 
-// The order of the table: most work first.  order: n entries
+// Two groups, each with its own table and launches.
+//   wide (n >= 2 m): the polynomial of two or three steps is taken on the Gram matrix, 13 m^3 + 6 m^2 n instead of 5 m^3 + 15 m^2 n flops
+//   others: every step goes back to X.  On the Gram matrix small singular values carry the rounding of the large ones' squares, and a square
+//   matrix has small ones: 3e-6 of the result instead of 5e-7 (64 x 64 noise; 1.1e-6 in plain float32), for no flops saved.
+int or_group(const aadg_matrix& a) {
+    const int64_t m = a.rows < a.cols ? a.rows : a.cols, n = (int64_t)a.rows + a.cols - m;
+    return n >= 2 * m ? 1 : 0;
+}
+
+// The order of a group's table: most work first.  order: room for n entries; the number filled is returned
 int64_t or_work(const aadg_matrix& a) {
     const int64_t m = a.rows < a.cols ? a.rows : a.cols;
     return m * ((int64_t)a.rows * a.cols + m * m);
 }
-void or_order(const aadg_matrix* mats, int n, int* order) {
-    for (int i = 0; i < n; ++i) order[i] = i;
-    std::sort(order, order + n, [&](int x, int y) { return or_work(mats[x]) != or_work(mats[y]) ? or_work(mats[x]) > or_work(mats[y]) : x < y; });
+int or_order(const aadg_matrix* mats, int n, int group, int* order) {
+    int k = 0;
+    for (int i = 0; i < n; ++i)
+        if (or_group(mats[i]) == group) order[k++] = i;
+    std::sort(order, order + k, [&](int x, int y) { return or_work(mats[x]) != or_work(mats[y]) ? or_work(mats[x]) > or_work(mats[y]) : x < y; });
+    return k;
 }
 
-// 0 or an error; fills the entries if `out` is given (n entries, matrix order[i] at i)
-int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out, const int* order) {
+int or_check(const aadg_matrix* mats, int n) {
     if (mats == nullptr || n < 1 || n > OR_MAX_MATS) return AADG_E_BADARG;
     for (int i = 0; i < n; ++i) {
         if (mats[i].rows < 1 || mats[i].cols < 1) return AADG_E_BADARG;
         if (mats[i].rows > OR_MAX_SIDE || mats[i].cols > OR_MAX_SIDE || (long long)mats[i].rows * mats[i].cols > (1 << 28)) return AADG_E_UNSUPPORTED;
     }
+    return 0;
+}
+
+// layout of a group behind byte `base` of the workspace: matrices order[0 .. k - 1]; fills the entries if `out` is given
+int or_layout(const aadg_matrix* mats, const int* order, int k, size_t base, OrLayout& lay, OrMat* out) {
     // tiles of 128 (twice the products per LDS byte of 64) where a phase then still has a workgroup for every CU
     long long sym = 0, rect = 0;
-    for (int i = 0; i < n; ++i) {
-        const long long m = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, k = (m + 127) / 128;
-        sym += k * (k + 1) / 2;
-        rect += k * (((long long)mats[i].rows + mats[i].cols - m + 127) / 128);
+    for (int i = 0; i < k; ++i) {
+        const aadg_matrix& a = mats[order[i]];
+        const long long m = a.rows < a.cols ? a.rows : a.cols, t = (m + 127) / 128;
+        sym += t * (t + 1) / 2;
+        rect += t * (((long long)a.rows + a.cols - m + 127) / 128);
     }
+    lay.n = k;
     lay.tb_sym = sym >= 256 ? 128 : 64;
     lay.tb_x = rect >= 256 ? 128 : 64;
     sym = 0;
-    for (int i = 0; i < n; ++i) {
-        const long long m = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, k = (m + lay.tb_sym - 1) / lay.tb_sym;
-        sym += k * (k + 1) / 2;
+    for (int i = 0; i < k; ++i) {
+        const aadg_matrix& a = mats[order[i]];
+        const long long m = a.rows < a.cols ? a.rows : a.cols, t = (m + lay.tb_sym - 1) / lay.tb_sym;
+        sym += t * (t + 1) / 2;
     }
     // pieces of the long axis: about two workgroups per CU, at least 512 values each (16 stages, as long as the join takes)
-    const long long pieces = sym >= 512 ? 1 : (512 + sym - 1) / sym;
-    size_t at = aadg_align_up((size_t)n * sizeof(OrMat), 256);
+    const long long pieces = sym >= 512 ? 1 : sym > 0 ? (512 + sym - 1) / sym : 1;
+    size_t at = base + aadg_align_up((size_t)k * sizeof(OrMat), 256);
     for (int p = 0; p < OR_PHASES; ++p) lay.grid[p] = 0;
     lay.split = false;
-    for (int i = 0; i < n; ++i) {
-        const aadg_matrix& a = mats[order != nullptr ? order[i] : i];
+    for (int i = 0; i < k; ++i) {
+        const aadg_matrix& a = mats[order[i]];
         OrMat t = {};
         t.src = a.src; t.dst = a.dst; t.rows = a.rows; t.cols = a.cols;
         t.m = t.rows < t.cols ? t.rows : t.cols;
@@ -512,7 +532,7 @@ int or_layout(const aadg_matrix* mats, int n, OrLayout& lay, OrMat* out, const i
         }
         if (out != nullptr) out[i] = t;
     }
-    lay.bytes = at;
+    lay.bytes = at - base;
     return 0;
 }
 
@@ -545,10 +565,11 @@ struct OrRun {
     }
 };
 
-int or_steps(const OrRun& run, int steps, float a, float b, float c) {
+// group 1: blocks of two and three steps on the Gram matrix; group 0: blocks of one
+int or_steps(const OrRun& run, int group, int steps, float a, float b, float c) {
     int x = OR_B_X0, y = OR_B_X1;
     for (int done = 0; done < steps;) {
-        const int block = steps - done < (done == 0 ? 2 : 3) ? steps - done : (done == 0 ? 2 : 3);
+        const int most = group == 0 ? 1 : done == 0 ? 2 : 3, block = steps - done < most ? steps - done : most;
         done += block;
         run.gram(x);
         int p = OR_B_P0, p2 = OR_B_P1, q = -1, free_q = OR_B_Q;                // q: the product of the block's P so far
@@ -583,40 +604,69 @@ int or_steps(const OrRun& run, int steps, float a, float b, float c) {
 
 }  // namespace
 
+// the two groups' layouts, the second behind the first.  order: 2 n ints of scratch, the groups' matrices in table order
+static int or_plan(const aadg_matrix* mats, int n, int* order, OrLayout* lay) {
+    size_t base = 0;
+    for (int g = 0; g < 2; ++g) {
+        const int rc = or_layout(mats, order + g * n, or_order(mats, n, g, order + g * n), base, lay[g], nullptr);
+        if (rc != 0) return rc;
+        base += lay[g].bytes;
+    }
+    return 0;
+}
+
 extern "C" size_t aadg_orthogonalize_workspace_bytes(const aadg_matrix* mats_host, int n) {
-    OrLayout lay;
-    return or_layout(mats_host, n, lay, nullptr, nullptr) == 0 ? lay.bytes : 0;
+    if (or_check(mats_host, n) != 0) return 0;
+    int* order = (int*)malloc((size_t)n * 2 * sizeof(int));
+    if (order == nullptr) return 0;
+    OrLayout lay[2];
+    const int rc = or_plan(mats_host, n, order, lay);
+    free(order);
+    return rc == 0 ? lay[0].bytes + lay[1].bytes : 0;
 }
 
 extern "C" int aadg_orthogonalize_f32(const aadg_matrix* mats_host, int n, int steps, float a, float b, float c, float eps, void* ws,
                                       size_t ws_bytes, void* stream) {
-    OrLayout lay;
-    const int rc = or_layout(mats_host, n, lay, nullptr, nullptr);
+    int rc = or_check(mats_host, n);
     if (rc != 0) return rc;
     if (steps < 1 || steps > 64 || !(eps >= 0.0f)) return AADG_E_BADARG;
     for (int i = 0; i < n; ++i)
         if (mats_host[i].src == nullptr || mats_host[i].dst == nullptr || (uintptr_t)mats_host[i].src % 4 != 0 || (uintptr_t)mats_host[i].dst % 4 != 0)
             return AADG_E_BADARG;
-    if (ws == nullptr || (uintptr_t)ws % 256 != 0 || ws_bytes < lay.bytes) return AADG_E_WORKSPACE;
-    OrMat* entries = (OrMat*)malloc((size_t)n * (sizeof(OrMat) + sizeof(int)));
+    OrMat* entries = (OrMat*)malloc((size_t)n * (sizeof(OrMat) + 2 * sizeof(int)));
     if (entries == nullptr) return AADG_E_WORKSPACE;
     int* order = (int*)(entries + n);
-    or_order(mats_host, n, order);
-    or_layout(mats_host, n, lay, entries, order);
+    OrLayout lay[2];
+    rc = or_plan(mats_host, n, order, lay);
+    if (rc == 0 && (ws == nullptr || (uintptr_t)ws % 256 != 0 || ws_bytes < lay[0].bytes + lay[1].bytes)) rc = AADG_E_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
-    OrMat* table = (OrMat*)ws;
-    constexpr int PER = OR_CHUNK;
-    static_assert(sizeof(OrChunk) + sizeof(OrMat*) <= 4096, "kernel arguments");
-    for (int i = 0; i < n; i += PER) {
-        OrChunk chunk = {};
-        chunk.base = i;
-        chunk.count = n - i < PER ? n - i : PER;
-        memcpy(chunk.mat, entries + i, (size_t)chunk.count * sizeof(OrMat));
-        hipLaunchKernelGGL(k_or_table, dim3(1), dim3(256), 0, st, chunk, table);
+    size_t base = 0;
+    // every matrix is read (norms, planes) before any result is written: dst may be another group's src
+    for (int pass = 0; pass < 2 && rc == 0; ++pass) {
+        base = 0;
+        for (int g = 0; g < 2 && rc == 0; ++g) {
+            const int k = lay[g].n;
+            OrMat* table = (OrMat*)((char*)ws + base);
+            if (k > 0 && pass == 0) {
+                or_layout(mats_host, order + g * n, k, base, lay[g], entries);
+                for (int i = 0; i < k; i += OR_CHUNK) {
+                    static_assert(sizeof(OrChunk) + sizeof(OrMat*) <= 4096, "kernel arguments");
+                    OrChunk chunk = {};
+                    chunk.base = i;
+                    chunk.count = k - i < OR_CHUNK ? k - i : OR_CHUNK;
+                    memcpy(chunk.mat, entries + i, (size_t)chunk.count * sizeof(OrMat));
+                    hipLaunchKernelGGL(k_or_table, dim3(1), dim3(256), 0, st, chunk, table);
+                }
+                hipLaunchKernelGGL(k_or_sum, dim3((unsigned)lay[g].grid[OR_P_SUM]), dim3(256), 0, st, table, k, (char*)ws);
+                hipLaunchKernelGGL(k_or_planes, dim3((unsigned)lay[g].grid[OR_P_SPLIT]), dim3(256), 0, st, table, k, (char*)ws, eps);
+                const hipError_t e = hipGetLastError();
+                if (e != hipSuccess) rc = (int)e;
+            } else if (k > 0) {
+                rc = or_steps(OrRun{lay[g], table, k, (char*)ws, st}, g, steps, a, b, c);
+            }
+            base += lay[g].bytes;
+        }
     }
     free(entries);
-    hipLaunchKernelGGL(k_or_sum, dim3((unsigned)lay.grid[OR_P_SUM]), dim3(256), 0, st, table, n, (char*)ws);
-    hipLaunchKernelGGL(k_or_planes, dim3((unsigned)lay.grid[OR_P_SPLIT]), dim3(256), 0, st, table, n, (char*)ws, eps);
-    AADG_LAUNCH_CHECK();
-    return or_steps(OrRun{lay, table, n, (char*)ws, st}, steps, a, b, c);
+    return rc;
 }
