@@ -65,6 +65,15 @@ template <> struct At<uint16_t> {
                             aadg_f2bf_pk(c[8 * g + 4], c[8 * g + 5]), aadg_f2bf_pk(c[8 * g + 6], c[8 * g + 7])};
         return __builtin_bit_cast(Frag, p);
     }
+    // what pack() rounds off
+    static __device__ __forceinline__ Frag rest(const f32x16& c, int g) {
+        const at_u32x4 x = __builtin_bit_cast(at_u32x4, pack(c, g));
+        at_u32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            y[i] = aadg_f2bf_pk(c[8 * g + 2 * i] - __uint_as_float(x[i] << 16), c[8 * g + 2 * i + 1] - __uint_as_float(x[i] & 0xFFFF0000u));
+        return __builtin_bit_cast(Frag, y);
+    }
     static __device__ __forceinline__ float dot(Frag a, Frag b, float s) {
         const at_u32x4 x = __builtin_bit_cast(at_u32x4, a), y = __builtin_bit_cast(at_u32x4, b);
 #pragma unroll
@@ -367,7 +376,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AtArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// D_i = do_i . o_i, one 16-lane group per row (only where dq, whose kernel computes it on the way, is not asked for)
+// D_i = do_i . o_i, one 16-lane group per row, where dq, whose kernel leaves it, is not asked for and no row can need its correction
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
     const long long rows = (long long)a.B * a.G * a.R, flat = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -385,7 +394,13 @@ __global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
     if ((threadIdx.x & 15) == 0) a.delta[flat] = s;
 }
 
-// dq: the forward's walk over the keys with p recomputed; dq^T += K^T ds^T
+// dq: the forward's walk over the keys with p recomputed; dq^T += K^T ds^T.  Leaves D_i for the dk / dv kernels.
+// D_i = do_i . o_i carries o's rounding (half a bfloat16 step of |do||o|).  With few keys that is not small beside dp_j - D_i: for bfloat16 rows of
+// up to 32 keys sum_j p_ij (dp_ij - D_i), zero but for that rounding, is added to D_i before the walk (two keys: gradients off by
+// 0.0024 of their size, not 0.0045; ten: 0.0027, 0.0032).
+// dS is rounded to the tensors' type for its products (2^-9 of each term, which the sum over keys or rows averages: about the size of the result's own
+// rounding).  Sequences of up to 32 keys, where few terms are averaged, and heads of up to 32 values, where D_i's rounding is largest beside dS,
+// take what bfloat16 rounds off as a second product.
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(const AtArgs a) {
     typedef At<T> M;
@@ -401,7 +416,7 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
     const int row0 = tile * 32 * NW + 32 * wv, row = row0 + (lane & 31);
     const bool live = row < a.R;
     const int k_lo = SPLIT ? sp * a.chunk : 0;
-    const int wg_end = min(at_limit_max(a, L, tile * 32 * NW, 32 * NW), SPLIT ? k_lo + a.chunk : L);
+    const int wg_end = min(at_limit_max(a, L, tile * 32 * NW, 32 * NW), SPLIT ? k_lo + a.chunk : a.dq == nullptr ? BK : L);      // (no dq: only D_i)
     const int limit = live ? at_limit(a, L, row) : 0;
     const int wave_end = row0 < a.R ? at_limit_max(a, L, row0, 32) : 0;
     int wave_full = limit;
@@ -429,7 +444,6 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
         for (int u = 0; u < U; ++u)
             dl = M::dot(__builtin_bit_cast(typename M::Frag, at_load<T>(yp, 0, live ? 0 : 1, 1, 2 * u + h, a.d)), gf[u], dl);
         dl += __shfl_xor(dl, 32, 64);
-        if (live && h == 0 && sp == 0) a.delta[flat] = dl;
     }
     const float c = a.scale * AT_LOG2E;
     f32x16 acc[DT];
@@ -460,6 +474,24 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
         if (k0 + BK < wg_end) fetch(k0 + BK);
         if (k0 >= wave_end) continue;
         const bool edge = k0 + BK > wave_full;
+        if (sizeof(T) == 2 && k0 == 0 && wave_full <= 32) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[i] = 0.0f;
+                dp[i] = -dl;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s = M::mma(L_::rows(Ks, 0, u, lane), qf[u], s);
+                dp = M::mma(L_::rows(Vs, 0, u, lane), gf[u], dp);
+            }
+            float fix = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) fix += 8 * (i >> 2) + 4 * h + (i & 3) < limit ? at_exp2(fmaf(s[i], c, -lse)) * dp[i] : 0.0f;
+            fix += __shfl_xor(fix, 32, 64);
+            dl += limit <= 32 ? fix : 0.0f;
+        }
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             f32x16 s, dp;
@@ -484,10 +516,18 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
                 const typename M::Frag pf = M::pack(s, p);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[dt] = M::mma(L_::cols(Ks, 32 * t + KS * p, 32 * dt, lane), pf, acc[dt]);
+                if constexpr (sizeof(T) == 2) {
+                    if (D > 32 && L > 32) continue;
+                    const typename M::Frag rf = M::rest(s, p);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) acc[dt] = M::mma(L_::cols(Ks, 32 * t + KS * p, 32 * dt, lane), rf, acc[dt]);
+                }
             }
         }
     }
     if (!live) return;
+    if (h == 0 && sp == 0) a.delta[flat] = dl;
+    if (a.dq == nullptr) return;
     const float sc = a.scale;
     T* op = (T*)a.dq + at_row(a, a.sdq, b, g, row);
     float* pp = SPLIT ? a.part + (sp * ((long long)a.B * a.G * a.R) + flat) * a.d : nullptr;
@@ -631,6 +671,12 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
                     av[dt] = M::mma(L_::cols(Gs, 32 * t + KS * p, 32 * dt, lane), pf, av[dt]);
                     ak[dt] = M::mma(L_::cols(Qs, 32 * t + KS * p, 32 * dt, lane), df, ak[dt]);
                 }
+                if constexpr (sizeof(T) == 2) {
+                    if (D > 32 && L > 32) continue;
+                    const typename M::Frag rf = M::rest(dp, p);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) ak[dt] = M::mma(L_::cols(Qs, 32 * t + KS * p, 32 * dt, lane), rf, ak[dt]);
+                }
             }
         }
         q0 = qn;
@@ -664,7 +710,7 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
 // S = Q K^T, makes P and hands it over through LDS (lane to lane, float32), then accumulates dv^T += dO^T P; wave 1 keeps V, takes dP = dO V^T - D
 // (-D_i is the initial value of its accumulators), makes dS = P dP and accumulates dk^T += Q^T dS.  Both halves are the same code on swapped
 // operands and the same number of products; one wave doing both needs 2 D accumulator and D fragment registers and leaves a SIMD one
-// wave (D = 128: 423 us instead of XXX us for two sequences of 4096, 8 heads).
+// wave (two causal sequences of 4096, 8 heads over 2, D = 128: 365 us, 423 in one wave).
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
     typedef At<T> M;
@@ -797,6 +843,12 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
                 const typename M::Frag pf = M::pack(s[t], p);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[dt] = M::mma(L_::cols(X2, 32 * t + KS * p, 32 * dt, lane), pf, acc[dt]);
+                if constexpr (sizeof(T) == 2) {
+                    if (L > 32) continue;
+                    const typename M::Frag rf = M::rest(s[t], p);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) acc[dt] = M::mma(L_::cols(X2, 32 * t + KS * p, 32 * dt, lane), rf, acc[dt]);
+                }
             }
         q0 = qn;
     }
@@ -939,6 +991,15 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_bwd_short(const AtArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+        if (wv == 0 && __any(Es[lane & 31] <= 32)) {                          // rows whose keys are all this wave's: D_i corrected as in k_attn_dq
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float fix = dp[i];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) fix += __shfl_xor(fix, o, 64);
+                dp[i] -= Es[8 * (i >> 2) + 4 * h + (i & 3)] <= 32 ? s[i] * fix : 0.0f;
+            }
+        }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             const typename M::Frag pf = M::pack(s, p), df = M::pack(dp, p);
@@ -1164,10 +1225,11 @@ template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, h
         AADG_LAUNCH_CHECK();
         return p.splits > 1 ? at_sum_kv<T>(a, p.splits, st) : 0;
     }
-    if (a.dq != nullptr) {
-        const AtPlan p = at_plan_rows(s);
+    if (a.dq != nullptr || (sizeof(T) == 2 && (a.causal || a.key_lengths != nullptr || a.Nk <= 32))) {
+        AtPlan p = at_plan_rows(s);
+        if (a.dq == nullptr) p.splits = 1;                                    // only for D_i
         at_use(a, p);
-        AT_BY_D(k_attn_dq, T, k_attn_dq, 1);                                                // leaves D_i in a.delta
+        AT_BY_D(k_attn_dq, T, k_attn_dq, 1);
         AADG_LAUNCH_CHECK();
         if (p.splits > 1) {
             const long long n = rows * (a.d / 4);

@@ -16,7 +16,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
-def definition(q, k, v, scale, causal, lengths, do=None):
+def definition(q, k, v, scale, causal, lengths, do=None, few_keys=False):
     """o, (dq, dk, dv) and their error bounds, in float64."""
     dt = q.dtype
     t, u = torch.finfo(dt).eps / 2, 2.0 ** -24
@@ -48,7 +48,11 @@ def definition(q, k, v, scale, causal, lengths, do=None):
     mag = dP.abs() + D.abs()
     dS = P * (dP - D)
     D_err = (g.abs() * o_err).sum(3, keepdim=True) + u * (d + 2) * (g.abs() * o.abs()).sum(3, keepdim=True)
-    dS_err = P * (e * mag + u * (d + 2) * torch.matmul(g.abs(), VT.abs()) + D_err + 4 * u * mag) + t * dS.abs()
+    ts = t
+    if few_keys:                                                            # D_i = sum_j p_ij dp_ij, none of o's rounding in it; dS in two terms
+        ts = t if 32 < Nk <= 256 and 32 < d <= 64 else t * t
+        D_err = (P * ((e + u * (Nk + 8)) * mag + u * (d + 2) * torch.matmul(g.abs(), VT.abs()))).sum(3, keepdim=True)
+    dS_err = P * (e * mag + u * (d + 2) * torch.matmul(g.abs(), VT.abs()) + D_err + 4 * u * mag) + ts * dS.abs()
     fold = lambda x: x.view(B, G, r, Nk, d).sum(2)                                              # noqa: E731  heads that share a key head
     tr = lambda x: x.transpose(2, 3).contiguous()                                               # noqa: E731
     dq, dk, dv = scale * torch.matmul(dS, K), fold(scale * torch.matmul(tr(dS), Q)), fold(torch.matmul(tr(P), g))
@@ -120,6 +124,32 @@ def test_attention_and_gradients_match_the_definition(hip, dtype, shape):
     if lens is not None:                                                    # keys behind the length: exactly zero
         for b in range(B):
             assert not grads[1][b, :, lens[b]:].any() and not grads[2][b, :, lens[b]:].any()
+
+
+@pytest.mark.parametrize("shape", [
+    (1, 1, 1, 1, 1, 8, False, None),                        # one key: dq = dk = 0 but for float32's roundings
+    (2, 4, 2, 17, 2, 24, True, None),
+    (1, 5, 5, 400, 3, 16, False, None),
+    (2, 4, 1, 130, 9, 128, False, [9, 2]),
+    (3, 2, 2, 31, 32, 64, True, [32, 5, 0]),
+    (2, 2, 2, 200, 32, 32, False, [32, 3]),
+    (3, 2, 2, 70, 200, 64, False, [4, 1, 32]),              # every key in one workgroup, few of them in use
+    (2, 4, 2, 32, 100, 48, True, [32, 17]),
+    (2, 2, 1, 50, 900, 40, False, [2, 30]),                 # a long cache, few of its keys in use: split over the keys
+])
+def test_gradients_of_few_keys_do_not_carry_the_rounding_of_the_output(hip, shape):
+    B, H, G, Nq, Nk, d, causal, lens = shape
+    q, k, v, do = inputs(torch.bfloat16, B, H, G, Nq, Nk, d, seed=11)
+    lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = definition(q, k, v, d ** -0.5, causal, lengths, do, few_keys=True)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    o = hip.attention(q, k, v, causal=causal, key_lengths=lengths)
+    for name, g, w in zip(("dq", "dk", "dv"), torch.autograd.grad(o, (q, k, v), do), want[1:]):
+        check(g, w, name)
+    o = hip.attention(q.detach(), k, v, causal=causal, key_lengths=lengths)
+    for name, g, w in zip(("dk", "dv"), torch.autograd.grad(o, (k, v), do), want[2:]):          # without dq
+        check(g, w, name)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
