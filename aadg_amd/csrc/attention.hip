@@ -194,6 +194,12 @@ template <typename T, int D, int NW> constexpr int at_bk() { return NW == 1 || (
 
 // ------------------------------------------------------------------------------------------------ forward
 // Workgroup: NW waves of 32 folded rows; keys in tiles of BK through LDS, the next tile's loads in registers during the products.
+// Bound by the vector units in bfloat16: a score costs as many of their cycles (exponential, maximum, sum, packing) as D / 32 matrix
+// instructions' share.  48 x 16384 rows, 256 keys, D = 64: 98 us, 0.53 PFLOP/s (vector issue 0.66 of the time, matrix 0.26); two causal sequences of
+// 8192, 16 heads over 4, D = 128: 800 us, 0.69 PFLOP/s (0.51, 0.41).  In float32 by the matrix units: 240 x 1024 rows, 256 keys, D = 64: 157 us,
+// 103 TFLOP/s of the 153 that a large float32 product reaches.  A workgroup that holds all 256
+// keys takes 88 us for the first case, but there is one to a CU and rows are cut into whole rounds of them (96 groups: 3/4 of the CUs), so this form
+// serves every shape.  Two row blocks a wave take the same time.
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_fwd(const AtArgs a) {
     typedef At<T> M;
@@ -398,9 +404,10 @@ __global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
 // D_i = do_i . o_i carries o's rounding (half a bfloat16 step of |do||o|).  With few keys that is not small beside dp_j - D_i: for bfloat16 rows of
 // up to 32 keys sum_j p_ij (dp_ij - D_i), zero but for that rounding, is added to D_i before the walk (two keys: gradients off by
 // 0.0024 of their size, not 0.0045; ten: 0.0027, 0.0032).
-// dS is rounded to the tensors' type for its products (2^-9 of each term, which the sum over keys or rows averages: about the size of the result's own
-// rounding).  Sequences of up to 32 keys, where few terms are averaged, and heads of up to 32 values, where D_i's rounding is largest beside dS,
+// dS is rounded to the tensors' type for its products (at most 2^-8 of each term, which the sum over keys or rows averages: about the size of the
+// result's own rounding).  Sequences of up to 32 keys, where few terms are averaged, and heads of up to 32 values, where D_i's rounding is largest beside dS,
 // take what bfloat16 rounds off as a second product.
+// Three products a pair like the forward's two: two causal sequences of 4096, 8 heads over 2, D = 128: 182 us, 0.57 PFLOP/s.
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(const AtArgs a) {
     typedef At<T> M;
@@ -552,6 +559,7 @@ __device__ __forceinline__ int at_key_tile(const AtArgs& a, int rank) {
 
 // dk, dv: a wave owns 32 keys (its K and V fragments stay in registers) and walks the folded rows, BQ at a time through LDS;
 // dv^T += dO^T P, dk^T += Q^T dS.  -D_i is the initial value of the dP accumulators.  (Head widths up to 64.)
+// 48 x 16384 rows, 256 keys, D = 64, bfloat16: 172 us, 0.60 PFLOP/s (vector units; k_attn_dq 139 more: k_attn_bwd_short needs 206 for both).
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(const AtArgs a) {
     typedef At<T> M;
@@ -875,6 +883,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
 // ([key][row], 72 bytes a key: 8-byte writes of neighbouring keys and the transpose reads spread over the banks), and dq^T = K^T dS^T is taken in
 // 16 x 16 tiles (v_mfma_f32_16x16x32_bf16: every wave has its tiles over all keys, no sum across waves; its K^T fragments stay in registers).
 // D_i comes from the rows on their way to LDS (eight neighbouring lanes hold a row).
+// 48 x 16384 rows, 256 keys, D = 64: 206 us, 0.63 PFLOP/s (139 + 172 us in two walks); vector issue 0.42, LDS 0.40, matrix 0.33 of the time: two
+// barriers a tile of 32 rows, which software pipelining over one barrier did not shorten.
 template <int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void k_attn_bwd_short(const AtArgs a) {
     typedef uint16_t T;
