@@ -192,11 +192,30 @@ template <typename T, int D> constexpr int at_min_waves() { return D == 128 ? 1 
 // keys per LDS tile: 64; 32 where the next tile's prefetch registers (2 BK D / threads values) would not fit beside the accumulators
 template <typename T, int D, int NW> constexpr int at_bk() { return NW == 1 || (sizeof(T) == 4 && D == 128) ? 32 : 64; }
 
+// group and row tile of a workgroup.  Causal: by the length of the tiles' rows, all groups and heads side by side, the longest first, so that the
+// launch does not end in long tiles; where every workgroup has a place at once (two a CU, number i and i + 256) the second half backwards,
+// so that a CU has a long and a short one.  (Tiles of a head: the r heads' in turn, exact where Nq is a multiple of the tile.)
+__device__ __forceinline__ void at_row_tile(const AtArgs& a, int w, bool split, int& bg, int& tile) {
+    if (!a.causal || split) {
+        bg = w / a.tiles;
+        tile = w - bg * a.tiles;
+        return;
+    }
+    const int n = a.B * a.G, rank = w / n, half = (a.tiles + 1) / 2, per = a.tiles / a.r, rest = a.tiles - per * a.r;
+    bg = w - rank * n;
+    int i = gridDim.x > 512 || rank < half ? rank : a.tiles - 1 - (rank - half);
+    tile = per * a.r + i;
+    if (i < rest) return;
+    i -= rest;
+    const int q = i / a.r;
+    tile = (i - q * a.r) * per + per - 1 - q;
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 // Workgroup: NW waves of 32 folded rows; keys in tiles of BK through LDS, the next tile's loads in registers during the products.
 // Bound by the vector units in bfloat16: a score costs as many of their cycles (exponential, maximum, sum, packing) as D / 32 matrix
 // instructions' share.  48 x 16384 rows, 256 keys, D = 64: 98 us, 0.53 PFLOP/s (vector issue 0.66 of the time, matrix 0.26); two causal sequences of
-// 8192, 16 heads over 4, D = 128: 800 us, 0.69 PFLOP/s (0.51, 0.41).  In float32 by the matrix units: 240 x 1024 rows, 256 keys, D = 64: 157 us,
+// 8192, 16 heads over 4, D = 128: 607 us, 0.91 PFLOP/s (800 us with each head's tiles in a row).  In float32 by the matrix units: 240 x 1024 rows, 256 keys, D = 64: 157 us,
 // 103 TFLOP/s of the 153 that a large float32 product reaches.  A workgroup that holds all 256
 // keys takes 88 us for the first case, but there is one to a CU and rows are cut into whole rounds of them (96 groups: 3/4 of the CUs), so this form
 // serves every shape.  Two row blocks a wave take the same time.
@@ -210,7 +229,9 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_fwd(co
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int sp = SPLIT ? blockIdx.x % a.splits : 0;
     const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
-    const int bg = w / a.tiles, tile = a.tiles - 1 - (w - bg * a.tiles), b = bg / a.G, g = bg - b * a.G;      // causal: longest rows first
+    int bg, tile;
+    at_row_tile(a, w, SPLIT, bg, tile);
+    const int b = bg / a.G, g = bg - b * a.G;
     const int L = at_len(a, b);
     const int row0 = tile * 32 * NW + 32 * wv, row = row0 + (lane & 31);
     const bool live = row < a.R;
@@ -407,7 +428,7 @@ __global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
 // dS is rounded to the tensors' type for its products (at most 2^-8 of each term, which the sum over keys or rows averages: about the size of the
 // result's own rounding).  Sequences of up to 32 keys, where few terms are averaged, and heads of up to 32 values, where D_i's rounding is largest beside dS,
 // take what bfloat16 rounds off as a second product.
-// Three products a pair like the forward's two: two causal sequences of 4096, 8 heads over 2, D = 128: 182 us, 0.57 PFLOP/s.
+// Three products a pair like the forward's two: two causal sequences of 4096, 8 heads over 2, D = 128: 160 us, 0.64 PFLOP/s.
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(const AtArgs a) {
     typedef At<T> M;
@@ -418,7 +439,9 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int sp = SPLIT ? blockIdx.x % a.splits : 0;
     const int w = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
-    const int bg = w / a.tiles, tile = a.tiles - 1 - (w - bg * a.tiles), b = bg / a.G, g = bg - b * a.G;
+    int bg, tile;
+    at_row_tile(a, w, SPLIT, bg, tile);
+    const int b = bg / a.G, g = bg - b * a.G;
     const int L = at_len(a, b);
     const int row0 = tile * 32 * NW + 32 * wv, row = row0 + (lane & 31);
     const bool live = row < a.R;
@@ -550,11 +573,11 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(con
         }
 }
 
-// order of the key tiles: the ones most rows see (causal: the first) are dealt first, and the second half backwards, so that the two workgroups a
-// CU holds, number i and i + 256 of 512, are a long and a short one
+// order of the key tiles: the ones most rows see (causal: the first) first, and as in at_row_tile the second half backwards where every workgroup
+// has a place at once
 __device__ __forceinline__ int at_key_tile(const AtArgs& a, int rank) {
     const int half = (a.tiles + 1) / 2;
-    return !a.causal || rank < half ? rank : a.tiles - 1 - (rank - half);
+    return !a.causal || gridDim.x > 512 || rank < half ? rank : a.tiles - 1 - (rank - half);
 }
 
 // dk, dv: a wave owns 32 keys (its K and V fragments stay in registers) and walks the folded rows, BQ at a time through LDS;
@@ -718,7 +741,7 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
 // S = Q K^T, makes P and hands it over through LDS (lane to lane, float32), then accumulates dv^T += dO^T P; wave 1 keeps V, takes dP = dO V^T - D
 // (-D_i is the initial value of its accumulators), makes dS = P dP and accumulates dk^T += Q^T dS.  Both halves are the same code on swapped
 // operands and the same number of products; one wave doing both needs 2 D accumulator and D fragment registers and leaves a SIMD one
-// wave (two causal sequences of 4096, 8 heads over 2, D = 128: 365 us, 423 in one wave).
+// wave (two causal sequences of 4096, 8 heads over 2, D = 128: 264 us, 0.52 PFLOP/s; in pieces half as fine 365 us, 423 in one wave).
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
     typedef At<T> M;
@@ -1118,8 +1141,10 @@ struct AtPlan { int nw, tiles, splits, chunk; };
 // Waves per workgroup by what there is to own (32 rows a wave).  Splits of the other axis, in units of `tile`, until the card has eight waves per
 // CU.  The join is a launch of its own (4 us), so a split keeps what takes as long: 256 / D tiles in bfloat16 (1 us a tile at D = 64), two at
 // D = 32 and one otherwise in float32 (5 us at D = 64); two where nearly nothing else runs (under a wave per four CUs) and a tile takes a
-// trip to memory, not its products.
-AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile, int small) {
+// trip to memory, not its products.  Causal key tiles differ in length: pieces of 2048 rows or more are cut twice as fine, so that a CU takes a new one
+// when a short one ends (dk and dv of two sequences of 4096, 8 heads over 2, D = 128: 264 us instead of 373, the join 5 us more; with shorter
+// pieces the join takes what that gains: 8 heads of 4096, D = 64: forward and backward 245 instead of 232).
+AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile, int small, bool keys) {
     AtPlan p;
     p.nw = own <= 32 * small ? small : 4;
     p.tiles = (own + 32 * p.nw - 1) / (32 * p.nw);
@@ -1128,6 +1153,8 @@ AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile, int s
     const int n = (other + tile - 1) / tile, least = waves < 64 && work > 2 ? 2 : work;
     int64_t sp = (AT_TARGET_WAVES + waves - 1) / waves;
     if (sp > n / least) sp = n / least;
+    if (keys && s->causal && sp < (2 * AT_TARGET_WAVES + waves - 1) / waves && sp < n / 64)
+        sp = std::min<int64_t>(n / 64, (2 * AT_TARGET_WAVES + waves - 1) / waves);
     if (sp > 64) sp = 64;
     if (sp < 1) sp = 1;
     const int per = (int)((n + sp - 1) / sp);
@@ -1135,11 +1162,11 @@ AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile, int s
     p.splits = (n + per - 1) / per;
     return p;
 }
-AtPlan at_plan_rows(const aadg_attention_desc* s) { return at_plan(s, s->H / s->G * s->Nq, s->Nk, 64, 1); }
+AtPlan at_plan_rows(const aadg_attention_desc* s) { return at_plan(s, s->H / s->G * s->Nq, s->Nk, 64, 1, false); }
 // (head widths over 64: a pair of waves has the 32 keys of a wave, so twice the keys are counted)
 AtPlan at_plan_keys(const aadg_attention_desc* s) {
     const int f = s->d > 64 ? 2 : 1;
-    return at_plan(s, f * s->Nk, s->H / s->G * s->Nq, 32, f);
+    return at_plan(s, f * s->Nk, s->H / s->G * s->Nq, 32, f, true);
 }
 
 // The one-walk backward: keys a workgroup can hold.  Splits of the rows by what they cost: a tile of 32 rows takes 2 us, the workgroups (one of eight
