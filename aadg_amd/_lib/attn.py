@@ -30,7 +30,7 @@ def _rows16(t):
 def _by_token(like):
     """[B, heads, n, d] tensor whose memory is [B, n, heads, d]: what the output projection reads and the input projections' gradients are."""
     B, h, n, d = like.shape
-    return torch.empty((B, n, h, d), dtype=like.dtype, device=like.device).transpose(1, 2)
+    return like.new_empty_strided((B, h, n, d), (n * h * d, d, h * d, 1))
 
 
 def _on(device):
@@ -88,15 +88,20 @@ class _Attention(torch.autograd.Function):
         return dq, dk if need_k else None, dv if need_v else None, None, None, None
 
 
-def attention_supported(q, k, v):
-    """True where `attention` takes these tensors: GPU, float32 / bfloat16, [B, H, Nq, d] and [B, G, Nk, d] with H % G == 0, d % 8 == 0, d <= 128."""
+def _fits(q, k, v):
     if not (q.is_cuda and q.dtype in _ATTN_DTYPES and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
         return False
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         return False
     (B, H, Nq, d), (Bk, G, Nk, dk) = q.shape, k.shape
-    if B != Bk or d != dk or G == 0 or H % G != 0 or d % 8 != 0 or not 0 < d <= 128:
+    return B == Bk and d == dk and G > 0 and H % G == 0 and d % 8 == 0 and 0 < d <= 128
+
+
+def attention_supported(q, k, v):
+    """True where `attention` takes these tensors: GPU, float32 / bfloat16, [B, H, Nq, d] and [B, G, Nk, d] with H % G == 0, d % 8 == 0, d <= 128."""
+    if not _fits(q, k, v):
         return False
+    (B, H, Nq, d), G, Nk = q.shape, k.shape[1], k.shape[2]
     return B * H * Nq * Nk == 0 or bool(load().aadg_attention_supported(_attn_desc(_ATTN_DTYPES[q.dtype], B, H, G, Nq, Nk, d, 0, 1.0)))
 
 
@@ -111,7 +116,7 @@ def attention(q, k, v, scale=None, causal=False, key_lengths=None):
     Returns [B, H, Nq, d] over [B, Nq, H, d] memory: `.transpose(1, 2).reshape(B, Nq, H * d)` is free.  Differentiable once in q, k, v."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise AadgError("aadg_amd kernels need GPU tensors (got %s, %s, %s); there is no CPU path" % (q.device, k.device, v.device))
-    if not attention_supported(q, k, v):
+    if not _fits(q, k, v):                                    # (sizes past the kernels' limits: the library refuses them)
         raise AadgError("attention: expected float32 / bfloat16 tensors of one type and device, q [B, H, Nq, d], k and v [B, G, Nk, d], H %% G == 0, "
                         "d %% 8 == 0, d <= 128; got %s %s %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
