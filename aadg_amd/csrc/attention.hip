@@ -1138,25 +1138,37 @@ bool at_aligned(const aadg_attention_desc* s, const void* p, const int64_t* st) 
 
 struct AtPlan { int nw, tiles, splits, chunk; };
 
-// Waves per workgroup by what there is to own (32 rows a wave).  Splits of the other axis, in units of `tile`, until the card has eight waves per
-// CU.  The join is a launch of its own (4 us), so a split keeps what takes as long: 256 / D tiles in bfloat16 (1 us a tile at D = 64), two at
-// D = 32 and one otherwise in float32 (5 us at D = 64); two where nearly nothing else runs (under a wave per four CUs) and a tile takes a
-// trip to memory, not its products.  Causal key tiles differ in length: pieces of 2048 rows or more are cut twice as fine, so that a CU takes a new one
+// Waves per workgroup by what there is to own (32 rows a wave).  Splits of the other axis, in units of `tile`.
+// bfloat16: until the card has eight waves per CU.  The join is a launch of its own (4 us), so a split keeps what takes as long: 256 / D tiles (1 us a
+// tile at D = 64); two where nearly nothing else runs (under a wave per four CUs) and a tile takes a trip to memory, not its
+// products.  Causal key tiles differ in length: pieces of 2048 rows or more are cut twice as fine, so that a CU takes a new one
 // when a short one ends (dk and dv of two sequences of 4096, 8 heads over 2, D = 128: 264 us instead of 373, the join 5 us more; with shorter
 // pieces the join takes what that gains: 8 heads of 4096, D = 64: forward and backward 245 instead of 232).
+// float32: one wave keeps a SIMD's matrix unit busy (a tile D / 20 us, a microsecond of latency), so the pieces run in rounds of one
+// workgroup of four per CU, or four of one; a split costs the join and its partials (written and read at 4.7 TB/s).  The cheapest by that count.
 AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile, int small, bool keys) {
     AtPlan p;
     p.nw = own <= 32 * small ? small : 4;
     p.tiles = (own + 32 * p.nw - 1) / (32 * p.nw);
-    const int64_t waves = (int64_t)s->B * s->G * p.tiles * p.nw;
-    const int D = s->d <= 32 ? 32 : s->d <= 64 ? 64 : 128, work = s->dtype == 1 ? 256 / D : D == 32 ? 2 : 1;
-    const int n = (other + tile - 1) / tile, least = waves < 64 && work > 2 ? 2 : work;
-    int64_t sp = (AT_TARGET_WAVES + waves - 1) / waves;
-    if (sp > n / least) sp = n / least;
-    if (keys && s->causal && sp < (2 * AT_TARGET_WAVES + waves - 1) / waves && sp < n / 64)
-        sp = std::min<int64_t>(n / 64, (2 * AT_TARGET_WAVES + waves - 1) / waves);
-    if (sp > 64) sp = 64;
-    if (sp < 1) sp = 1;
+    const int64_t bg = (int64_t)s->B * s->G, waves = bg * p.tiles * p.nw;
+    const int D = s->d <= 32 ? 32 : s->d <= 64 ? 64 : 128, n = (other + tile - 1) / tile;
+    int64_t sp = 1;
+    if (s->dtype == 1) {
+        const int least = waves < 64 && D < 128 ? 2 : 256 / D;
+        sp = std::min<int64_t>((AT_TARGET_WAVES + waves - 1) / waves, n / least);
+        if (keys && s->causal && sp < (2 * AT_TARGET_WAVES + waves - 1) / waves && sp < n / 64)
+            sp = std::min<int64_t>(n / 64, (2 * AT_TARGET_WAVES + waves - 1) / waves);
+        sp = std::max<int64_t>(1, std::min<int64_t>(sp, 64));
+    } else {
+        const double part = (keys ? 16.0 : 8.0) * bg * own * s->d / 4.7e6;
+        double best = 0.0;
+        for (int64_t x = 1; x <= 64 && x <= n; ++x) {
+            const double cost = (double)((waves * x + 1023) / 1024 * ((n + x - 1) / x)) * (D / 20.0 + 1.0) + (x > 1 ? 4.0 + part * x : 0.0);
+            if (x > 1 && cost >= best) continue;
+            best = cost;
+            sp = x;
+        }
+    }
     const int per = (int)((n + sp - 1) / sp);
     p.chunk = per * tile;
     p.splits = (n + per - 1) / per;
