@@ -100,6 +100,10 @@ SHAPES = [
     (3, 1, 1, 31, 33, 40, False, None),
     (2, 2, 2, 1030, 250, 56, False, [250, 129]),
     (300, 1, 1, 40, 129, 64, False, None),
+    # causal: more row tiles than places, tiles that do not divide by the shared heads; rows in long pieces
+    (130, 3, 1, 200, 150, 32, True, None),
+    (70, 6, 2, 300, 310, 72, True, None),
+    (128, 8, 2, 1540, 70, 24, True, None),
 ]
 
 
