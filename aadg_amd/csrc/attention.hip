@@ -427,7 +427,7 @@ __global__ __launch_bounds__(256) void k_attn_delta(const AtArgs a) {
 // 0.0024 of their size, not 0.0045; ten: 0.0027, 0.0032).
 // dS is rounded to the tensors' type for its products (at most 2^-8 of each term, which the sum over keys or rows averages: about the size of the
 // result's own rounding).  Sequences of up to 32 keys, where few terms are averaged, and heads of up to 32 values, where D_i's rounding is largest beside dS,
-// take what bfloat16 rounds off as a second product.
+// take what bfloat16 rounds off as a second product (every backward kernel: a sequence's gradients do not depend on its batch's padding).
 // Three products a pair like the forward's two: two causal sequences of 4096, 8 heads over 2, D = 128: 160 us, 0.64 PFLOP/s.
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dq(const AtArgs a) {
@@ -948,6 +948,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_bwd_short(const AtArgs a) {
         const at_u32x4 y = {x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16};
         kt[n] = __builtin_bit_cast(typename M::Frag, y);
     }
+    // up to 32 keys are all wave 0's: what bfloat16 rounds off dS takes the place of the empty keys 32 ... 63, beside the same K^T (wave 1 writes
+    // its zeros over wave 2's)
+    const bool few = L <= 32;
+    const int skey = few && wv == 1 ? key + 32 : key;
+    if (few) kt[1] = kt[0];
     f32x16 ak[DT], av[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -1037,12 +1042,23 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_bwd_short(const AtArgs a) {
         for (int p = 0; p < 2; ++p) {
             const typename M::Frag pf = M::pack(s, p), df = M::pack(dp, p);
             const at_u32x4 dw = __builtin_bit_cast(at_u32x4, df);             // rows 16 p + 4 h + 0 ... 3 and + 8
-            *reinterpret_cast<uint2*>(&Ss[key * SP + 16 * p + 4 * h]) = make_uint2(dw[0], dw[1]);
-            *reinterpret_cast<uint2*>(&Ss[key * SP + 16 * p + 8 + 4 * h]) = make_uint2(dw[2], dw[3]);
+            *reinterpret_cast<uint2*>(&Ss[skey * SP + 16 * p + 4 * h]) = make_uint2(dw[0], dw[1]);
+            *reinterpret_cast<uint2*>(&Ss[skey * SP + 16 * p + 8 + 4 * h]) = make_uint2(dw[2], dw[3]);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 av[dt] = M::mma(L_::cols(Gs, KS * p, 32 * dt, lane), pf, av[dt]);
                 ak[dt] = M::mma(L_::cols(Qs, KS * p, 32 * dt, lane), df, ak[dt]);
+            }
+        }
+        if (few && wv == 0) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const typename M::Frag rf = M::rest(dp, p);
+                const at_u32x4 dw = __builtin_bit_cast(at_u32x4, rf);
+                *reinterpret_cast<uint2*>(&Ss[(32 + key) * SP + 16 * p + 4 * h]) = make_uint2(dw[0], dw[1]);
+                *reinterpret_cast<uint2*>(&Ss[(32 + key) * SP + 16 * p + 8 + 4 * h]) = make_uint2(dw[2], dw[3]);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) ak[dt] = M::mma(L_::cols(Qs, KS * p, 32 * dt, lane), rf, ak[dt]);
             }
         }
         __syncthreads();

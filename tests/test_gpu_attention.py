@@ -338,3 +338,24 @@ def test_refusals(hip):
     g = torch.autograd.grad(hip.attention(x, k, v).sum(), x, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         g.sum().backward()                                                              # differentiable once
+
+
+@pytest.mark.parametrize("shape", [
+    # bfloat16, sequences of up to 32 keys in a batch padded to 33 ... 256: the gradients of the same sequences in a batch padded to 32
+    (3, 2, 2, 70, 200, 64, False, [4, 1, 32]),
+    (2, 4, 2, 90, 100, 48, True, [32, 17]),
+    (2, 1, 1, 1500, 256, 64, False, [31, 9]),               # rows split over workgroups
+    (40, 2, 1, 33, 33, 40, False, [1 + i % 32 for i in range(40)]),
+])
+def test_gradients_of_few_keys_do_not_depend_on_the_padding(hip, shape):
+    B, H, G, Nq, Nk, d, causal, lens = shape
+    q, k, v, do = inputs(torch.bfloat16, B, H, G, Nq, Nk, d, seed=17)
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    n = max(lens)
+    want = definition(q, k[:, :, :n], v[:, :, :n], d ** -0.5, causal, lengths, do, few_keys=True)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(hip.attention(*leaves, causal=causal, key_lengths=lengths), leaves, do)
+    check(grads[0], want[1], "dq")
+    for name, g, w in zip(("dk", "dv"), grads[1:], want[2:]):
+        check(g[:, :, :n], w, name)
+        assert not g[:, :, n:].any()
