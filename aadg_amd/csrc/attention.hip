@@ -616,6 +616,8 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
 #pragma unroll
         for (int i = 0; i < 16; ++i) ak[t][i] = av[t][i] = 0.0f;
     // first tile from q0 on with a row that sees a key of this workgroup
+    // rows that see no key have zeros in LDS, whatever q, dO and D hold (0 x NaN in the products otherwise)
+    const bool blind = a.causal && L < a.Nq;
     auto next = [&](int q0) {
         if (a.causal)
             while (q0 < r_hi && at_limit_max(a, L, q0, BQ) <= wg_key0) q0 += BQ;
@@ -642,15 +644,16 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
         for (int i = 0; i < LD; ++i) {
             const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
             if (BQ * CPR % NT != 0 && id >= BQ * CPR) break;
-            const bool ok = q0 + rw < r_hi && ch * CH < a.d;
+            const bool ok = q0 + rw < r_hi && ch * CH < a.d && (!blind || at_limit(a, L, q0 + rw) > 0);
             *reinterpret_cast<at_u32x4*>(&Qs[L_::at(rw, ch)]) = at_keep(rq[i], ok);
             *reinterpret_cast<at_u32x4*>(&Gs[L_::at(rw, ch)]) = at_keep(rg[i], ok);
         }
         if (tid < BQ) {
             const bool ok = q0 + tid < r_hi;
             Ls[tid] = ok ? r_lse : INFINITY;
-            Ds[tid] = ok ? -r_d : 0.0f;
-            Es[tid] = ok ? at_limit(a, L, q0 + tid) : 0;
+            const int e = ok ? at_limit(a, L, q0 + tid) : 0;
+            Ds[tid] = e > 0 ? -r_d : 0.0f;
+            Es[tid] = e;
         }
         __syncthreads();
         const int qn = next(q0 + BQ);
@@ -772,6 +775,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
     // first tile from q0 on with a row that sees a key of this workgroup
+    // rows that see no key have zeros in LDS, whatever q, dO and D hold (0 x NaN in the products otherwise)
+    const bool blind = a.causal && L < a.Nq;
     auto next = [&](int q0) {
         if (a.causal)
             while (q0 < r_hi && at_limit_max(a, L, q0, BQ) <= wg_key0) q0 += BQ;
@@ -802,15 +807,16 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
         for (int i = 0; i < LD; ++i) {
             const int id = tid + NT * i, rw = id / CPR, ch = id - rw * CPR;
             if (BQ * CPR % NT != 0 && id >= BQ * CPR) break;
-            const bool ok = q0 + rw < r_hi && ch * CH < a.d;
+            const bool ok = q0 + rw < r_hi && ch * CH < a.d && (!blind || at_limit(a, L, q0 + rw) > 0);
             *reinterpret_cast<at_u32x4*>(&Xs[L_::at(rw, ch)]) = at_keep(rq[i], ok);
             *reinterpret_cast<at_u32x4*>(&Xs[BQ * L_::PITCH + L_::at(rw, ch)]) = at_keep(rg[i], ok);
         }
         if (tid < BQ) {
             const bool ok = q0 + tid < r_hi;
             Ls[tid] = ok ? r_lse : INFINITY;
-            Ds[tid] = ok ? -r_d : 0.0f;
-            Es[tid] = ok ? at_limit(a, L, q0 + tid) : 0;
+            const int e = ok ? at_limit(a, L, q0 + tid) : 0;
+            Ds[tid] = e > 0 ? -r_d : 0.0f;
+            Es[tid] = e;
         }
         __syncthreads();
         const int qn = next(q0 + BQ);
@@ -973,10 +979,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_bwd_short(const AtArgs a) {
         r_lse = a.lse[((long long)b * a.G + g) * a.R + min(q0 + (tid & 31), r_hi - 1)];
     };
     const bool edge = a.causal || key0 + 32 > L;
+    const bool blind = L == 0 || (a.causal && L < a.Nq);                      // rows that see no key: zeros in LDS as in k_attn_dkv
     fetch(r_lo);
     for (int q0 = r_lo; q0 < r_hi; q0 += BQ) {
         // (the last reads of Qs, Gs lie before the barrier in the middle of the last tile, those of Ss before the next barrier)
-        const bool ok = q0 + rw < r_hi && ch * 8 < a.d;
+        const bool ok = q0 + rw < r_hi && ch * 8 < a.d && (!blind || at_limit(a, L, q0 + rw) > 0);
         if (has_q) *reinterpret_cast<at_u32x4*>(&Qs[L_::at(rw, ch)]) = at_keep(rq, ok);
         if (has_g) {
             const at_u32x4 x = at_keep(rg, ok);

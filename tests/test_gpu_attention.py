@@ -359,3 +359,40 @@ def test_gradients_of_few_keys_do_not_depend_on_the_padding(hip, shape):
     for name, g, w in zip(("dk", "dv"), grads[1:], want[2:]):
         check(g[:, :, :n], w, name)
         assert not g[:, :, n:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [
+    # sequences without a key, causal sequences with more queries than keys: every backward kernel
+    (3, 2, 1, 70, 200, 64, False, [200, 0, 64]),
+    (2, 2, 2, 257, 129, 64, True, None),
+    (2, 2, 1, 90, 100, 48, True, [100, 30]),
+    (2, 4, 2, 400, 300, 32, True, [300, 7]),
+    (2, 2, 1, 150, 100, 128, True, [100, 0]),
+    (1, 2, 1, 40, 9, 96, True, None),
+    (1, 2, 1, 40, 9, 16, True, None),
+    (2, 1, 1, 900, 500, 64, True, [500, 420]),
+])
+def test_queries_that_see_no_key_take_no_part_whatever_they_hold(hip, dtype, shape):
+    B, H, G, Nq, Nk, d, causal, lens = shape
+    q, k, v, do = inputs(dtype, B, H, G, Nq, Nk, d, seed=23)
+    L = [Nk] * B if lens is None else lens
+    lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    rows = [Nq if n == 0 else max(0, Nq - n) if causal else 0 for n in L]              # the first rows of a sequence see nothing
+
+    def run(fill, ask):
+        leaves = [t.clone() for t in (q, k, v)]
+        g = do.clone()
+        for b, n in enumerate(rows):
+            leaves[0][b, :, :n] = fill
+            g[b, :, :n] = fill
+        for i in ask:
+            leaves[i].requires_grad_(True)
+        o = hip.attention(*leaves, causal=causal, key_lengths=lengths)
+        return [o.detach(), *torch.autograd.grad(o, [leaves[i] for i in ask], g)]
+    assert any(rows)
+    for ask in ((0, 1, 2), (1, 2), (0,)):
+        want = run(0.0, ask)
+        for fill in (float("nan"), float("inf")):
+            got = run(fill, ask)
+            assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(got, want)), (ask, fill)
