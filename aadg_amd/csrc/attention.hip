@@ -1297,7 +1297,8 @@ template <typename T> int at_backward(AtArgs& a, const aadg_attention_desc* s, h
         AADG_LAUNCH_CHECK();
         return p.splits > 1 ? at_sum_kv<T>(a, p.splits, st) : 0;
     }
-    if (a.dq != nullptr || (sizeof(T) == 2 && (a.causal || a.key_lengths != nullptr || a.Nk <= 32))) {
+    // (k_attn_delta has 16 threads a row and a launch less than 2^32 of them)
+    if (a.dq != nullptr || rows >= 1ll << 28 || (sizeof(T) == 2 && (a.causal || a.key_lengths != nullptr || a.Nk <= 32))) {
         AtPlan p = at_plan_rows(s);
         if (a.dq == nullptr) p.splits = 1;                                    // only for D_i
         at_use(a, p);

@@ -396,3 +396,20 @@ def test_queries_that_see_no_key_take_no_part_whatever_they_hold(hip, dtype, sha
         for fill in (float("nan"), float("inf")):
             got = run(fill, ask)
             assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(got, want)), (ask, fill)
+
+
+def test_more_rows_than_one_launch_of_16_lanes_a_row_has_threads(hip):
+    """2^28 + 192 rows, gradients of keys and values only: 16 threads a row would be past the 2^32 threads of a launch.  All rows but the first and
+    the last 128 are zero in q and dO and add nothing."""
+    n, d, Nk = (1 << 28) + 192, 8, 40
+    q, k, v, do = inputs(torch.bfloat16, 1, 1, 1, 256, Nk, d, seed=4)
+    far = [torch.zeros(1, 1, n, d, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for f, t in zip(far, (q, do)):
+        f[:, :, :128] = t[:, :, :128]
+        f[:, :, n - 128:] = t[:, :, 128:]
+    want = definition(q, k, v, d ** -0.5, False, None, do)
+    leaves = [t.requires_grad_(True) for t in (k, v)]
+    o = hip.attention(far[0], *leaves)
+    check(torch.cat([o.detach()[:, :, :128], o.detach()[:, :, n - 128:]], 2), want[0], "o")
+    for name, g, w in zip(("dk", "dv"), torch.autograd.grad(o, leaves, far[1]), want[2:]):
+        check(g, w, name)
