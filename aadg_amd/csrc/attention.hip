@@ -1183,7 +1183,7 @@ AtPlan at_plan(const aadg_attention_desc* s, int own, int other, int tile, int s
             sp = std::min<int64_t>(n / 64, (2 * AT_TARGET_WAVES + waves - 1) / waves);
         sp = std::max<int64_t>(1, std::min<int64_t>(sp, 64));
     } else {
-        const double part = (keys ? 16.0 : 8.0) * bg * own * s->d / 4.7e6;
+        const double part = (keys ? 16.0 : 8.0) * bg * (own / small) * s->d / 4.7e6;      // (own / small: the rows or keys that are written)
         double best = 0.0;
         for (int64_t x = 1; x <= 64 && x <= n; ++x) {
             const double cost = (double)((waves * x + 1023) / 1024 * ((n + x - 1) / x)) * (D / 20.0 + 1.0) + (x > 1 ? 4.0 + part * x : 0.0);

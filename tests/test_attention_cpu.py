@@ -72,3 +72,24 @@ def test_attention_has_no_cpu_path():
     assert not _lib.attention_supported(q, q, q)
     with pytest.raises(_lib.AadgError):
         _lib.attention(q, q, q)
+
+
+@pytest.mark.parametrize("B,G,r,Nq,Nk,d", [(6, 1, 1, 3000, 3000, 128), (6, 1, 1, 3000, 3000, 64), (2, 2, 2, 700, 1500, 96), (1, 3, 1, 5000, 900, 72), (8, 2, 1, 1023, 517, 64)])
+def test_float32_splits_count_the_bytes_that_the_join_moves(B, G, r, Nq, Nk, d):
+    """The backward's workspace is D_i and the partials of dk, dv or of dq.  Splits, as at_plan states them: rounds of workgroups times the tiles of a
+    split (D / 20 + 1 us each), and for a join 4 us and the partials at 4.7 TB/s, written and read once: Nk keys, whatever number of waves owns them."""
+    from aadg_amd import _lib
+    D = 32 if d <= 32 else 64 if d <= 64 else 128
+
+    def splits(own, count, other, tile, small, tensors):
+        nw = small if own <= 32 * small else 4
+        waves, n = B * G * (-(-own // (32 * nw))) * nw, -(-other // tile)
+        part = 8.0 * tensors * B * G * count * d / 4.7e6
+        costs = [((waves * x + 1023) // 1024 * -(-n // x)) * (D / 20.0 + 1.0) + (4.0 + part * x if x > 1 else 0.0) for x in range(1, min(64, n) + 1)]
+        per = -(-n // (costs.index(min(costs)) + 1))
+        return -(-n // per)
+    f = 2 if d > 64 else 1
+    sk, sq = splits(f * Nk, Nk, r * Nq, 32, f, 2), splits(r * Nq, r * Nq, Nk, 64, 1, 1)
+    want = -(-B * G * r * Nq * 4 // 256) * 256 + max(sk * 2 * B * G * Nk * d * 4 if sk > 1 else 0, sq * B * G * r * Nq * d * 4 if sq > 1 else 0)
+    desc = _desc(_lib, dtype=0, B=B, H=G * r, G=G, Nq=Nq, Nk=Nk, d=d)
+    assert _lib.load().aadg_attention_backward_workspace_bytes(ctypes.byref(desc)) == want
