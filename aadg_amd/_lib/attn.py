@@ -4,6 +4,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .binding import AadgError, _check, _ptr, _stream, load
@@ -113,7 +114,8 @@ def attention(q, k, v, scale=None, causal=False, key_lengths=None):
     causal: query i of a sequence with L keys sees keys j <= i + L - Nq (the last query sees every key).  A query that sees no key
     gives zeros and takes no part in any gradient.  Inputs are expected finite (a key that only the causal rule hides included).
 
-    Returns [B, H, Nq, d] over [B, Nq, H, d] memory: `.transpose(1, 2).reshape(B, Nq, H * d)` is free.  Differentiable once in q, k, v."""
+    Returns [B, H, Nq, d] over [B, Nq, H, d] memory: `.transpose(1, 2).reshape(B, Nq, H * d)` is free.  Differentiable once in q, k, v, in reverse mode (a
+    forward-mode tangent raises NotImplementedError)."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise AadgError("aadg_amd kernels need GPU tensors (got %s, %s, %s); there is no CPU path" % (q.device, k.device, v.device))
     if not _fits(q, k, v):                                    # (sizes past the kernels' limits: the library refuses them)
@@ -125,7 +127,9 @@ def attention(q, k, v, scale=None, causal=False, key_lengths=None):
     if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (q.shape[0],) or not key_lengths.is_contiguous() or
                                     key_lengths.device != q.device):
         raise AadgError("attention: key_lengths must be a contiguous int32 vector with one length per sequence (%d) on %s" % (q.shape[0], q.device))
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) and q.numel() > 0 and k.numel() > 0:
+    # (inside a forward-mode level the call goes through autograd, which refuses tangents; the direct path would drop them)
+    if (not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) and q.numel() > 0 and k.numel() > 0 and
+            forward_ad._current_level < 0):
         with _on(q.device):
             return _attention_forward(q, k, v, scale, bool(causal), key_lengths, False)[3]
     return _Attention.apply(q, k, v, scale, bool(causal), key_lengths)

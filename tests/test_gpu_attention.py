@@ -413,3 +413,18 @@ def test_more_rows_than_one_launch_of_16_lanes_a_row_has_threads(hip):
     check(torch.cat([o.detach()[:, :, :128], o.detach()[:, :, n - 128:]], 2), want[0], "o")
     for name, g, w in zip(("dk", "dv"), torch.autograd.grad(o, leaves, far[1]), want[2:]):
         check(g, w, name)
+
+
+def test_forward_mode_derivatives_are_refused(hip):
+    """a tangent is not dropped"""
+    from torch.autograd import forward_ad
+    q, k, v, _ = inputs(torch.float32, 1, 2, 2, 9, 12, 64)
+    want = hip.attention(q, k, v)
+    with forward_ad.dual_level():
+        assert torch.equal(hip.attention(q, k, v), want)                                # no tangent anywhere
+        for i in range(3):
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if n == i else t for n, t in enumerate((q, k, v))]
+            with pytest.raises(NotImplementedError):
+                hip.attention(*args)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                hip.attention(*args)
