@@ -16,7 +16,10 @@ _NO_STRIDE = (0, 0, 0)
 
 def _attn_desc(dtype, B, H, G, Nq, Nk, d, causal, scale, *strides):
     flat = [x for st in strides for x in st[:3]]
-    return _ATTN_DESC.pack(dtype, B, H, G, Nq, Nk, d, causal, scale, 0, *flat, *(0,) * (24 - len(flat)))
+    try:
+        return _ATTN_DESC.pack(dtype, B, H, G, Nq, Nk, d, causal, scale, 0, *flat, *(0,) * (24 - len(flat)))
+    except (struct.error, OverflowError):                     # sizes past 32 bits, a scale past float32
+        raise AadgError("attention: sizes (%d, %d, %d, %d, %d, %d) or scale %r out of range" % (B, H, G, Nq, Nk, d, scale)) from None
 
 
 def _rows16(t):
@@ -103,6 +106,8 @@ def attention_supported(q, k, v):
     if not _fits(q, k, v):
         return False
     (B, H, Nq, d), G, Nk = q.shape, k.shape[1], k.shape[2]
+    if max(B, H, Nq, Nk) >= 1 << 31:
+        return False
     return B * H * Nq * Nk == 0 or bool(load().aadg_attention_supported(_attn_desc(_ATTN_DTYPES[q.dtype], B, H, G, Nq, Nk, d, 0, 1.0)))
 
 
@@ -124,8 +129,8 @@ def attention(q, k, v, scale=None, causal=False, key_lengths=None):
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise AadgError("attention: scale must be positive and finite, got %r" % scale)
-    if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != (q.shape[0],) or not key_lengths.is_contiguous() or
-                                    key_lengths.device != q.device):
+    if key_lengths is not None and (not torch.is_tensor(key_lengths) or key_lengths.dtype != torch.int32 or key_lengths.shape != (q.shape[0],) or
+                                    not key_lengths.is_contiguous() or key_lengths.device != q.device):
         raise AadgError("attention: key_lengths must be a contiguous int32 vector with one length per sequence (%d) on %s" % (q.shape[0], q.device))
     # (inside a forward-mode level the call goes through autograd, which refuses tangents; the direct path would drop them)
     if (not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) and q.numel() > 0 and k.numel() > 0 and

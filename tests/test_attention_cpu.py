@@ -93,3 +93,11 @@ def test_float32_splits_count_the_bytes_that_the_join_moves(B, G, r, Nq, Nk, d):
     want = -(-B * G * r * Nq * 4 // 256) * 256 + max(sk * 2 * B * G * Nk * d * 4 if sk > 1 else 0, sq * B * G * r * Nq * d * 4 if sq > 1 else 0)
     desc = _desc(_lib, dtype=0, B=B, H=G * r, G=G, Nq=Nq, Nk=Nk, d=d)
     assert _lib.load().aadg_attention_backward_workspace_bytes(ctypes.byref(desc)) == want
+
+
+@pytest.mark.parametrize("change", [dict(scale=1e39), dict(Nq=1 << 31), dict(B=1 << 33)])
+def test_descriptor_refuses_what_it_cannot_hold(change):
+    from aadg_amd import _lib
+    a = {**dict(dtype=0, B=1, H=1, G=1, Nq=8, Nk=8, d=8, causal=False, scale=1.0), **change}
+    with pytest.raises(_lib.AadgError):
+        _lib._attn_desc(*a.values())

@@ -428,3 +428,14 @@ def test_forward_mode_derivatives_are_refused(hip):
                 hip.attention(*args)
             with torch.no_grad(), pytest.raises(NotImplementedError):
                 hip.attention(*args)
+
+
+def test_sizes_and_scales_past_the_descriptor_are_refused(hip):
+    q, k, v, _ = inputs(torch.float32, 1, 1, 1, 8, 8, 8)
+    for kw in (dict(scale=1e39), dict(scale=1e-60), dict(key_lengths=[8]), dict(key_lengths=8)):
+        with pytest.raises(hip.AadgError):
+            hip.attention(q, k, v, **kw)
+    wide = k[:, :, :1].expand(1, 1, 1 << 31, 8)
+    assert not hip.attention_supported(q, wide, wide)
+    with pytest.raises(hip.AadgError):
+        hip.attention(q, wide, wide)
