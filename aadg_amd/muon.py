@@ -19,21 +19,43 @@ def is_matrix(p):
 
 
 class Muon(torch.optim.Optimizer):
-    """`params`: parameters on one GPU, split by `is_matrix` into a Muon and an Adam group (one learning rate, one decay).  `weight_decay` is
-    decoupled for the matrices and added to the gradient for the others, as in Adam.  Float32 parameters only."""
+    """`params`: parameters on one GPU, or groups of them as torch's optimisers take them.  Every group, one added later too, becomes a Muon and an
+    Adam group, split by `is_matrix` (one learning rate, one decay); `matrices=True / False` in a group puts all of it on one side.  Parameters that
+    require no gradient are left out.  `weight_decay` is decoupled for the matrices and added to the gradient for the others, as in Adam.
+    Float32 parameters only."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.0, momentum=0.95, betas=(0.9, 0.999), eps=1e-8, steps=5):
-        params = [p for p in params if p.requires_grad]
-        for p in params:
-            if not p.is_cuda:
-                raise _lib.AadgError("Muon: parameters must be on the GPU (got %s); there is no CPU path" % p.device)
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, betas=betas, eps=eps, steps=steps))
+
+    def add_param_group(self, param_group):
+        group = {**self.defaults, **param_group}
+        lr, wd, momentum, betas, eps, steps = (group[k] for k in ("lr", "weight_decay", "momentum", "betas", "eps", "steps"))
+        if (not lr >= 0.0 or not wd >= 0.0 or not 0.0 <= momentum < 1.0 or not all(0.0 <= b < 1.0 for b in betas) or not eps > 0.0 or
+                not (1 <= steps <= 64 and int(steps) == steps)):
+            raise ValueError("Muon: lr %r, weight_decay %r, momentum %r, betas %r, eps %r, steps %r" % (lr, wd, momentum, betas, eps, steps))
+        params = [group["params"]] if torch.is_tensor(group["params"]) else list(group["params"])
+        tensor = lambda p: p[1] if isinstance(p, tuple) else p                                  # noqa: E731  (name, parameter)
+        if not all(torch.is_tensor(tensor(p)) for p in params):
+            raise TypeError("Muon: parameters must be tensors")
+        params = [p for p in params if tensor(p).requires_grad]
+        if not params:
+            raise ValueError("Muon: no parameter of the group requires a gradient")
+        device = next((p.device for g in self.param_groups for p in g["params"]), tensor(params[0]).device)
+        for p in map(tensor, params):
+            if not p.is_cuda or p.device != device:
+                raise _lib.AadgError("Muon: parameters must be on one GPU (got %s, %s); there is no CPU path" % (p.device, device))
             if p.dtype != torch.float32:
                 raise _lib.AadgError("Muon: float32 parameters only, got %s" % p.dtype)
-        if not lr >= 0.0 or not weight_decay >= 0.0 or not 0.0 <= momentum < 1.0 or not all(0.0 <= b < 1.0 for b in betas) or not eps > 0.0:
-            raise ValueError("Muon: lr %r, weight_decay %r, momentum %r, betas %r, eps %r" % (lr, weight_decay, momentum, betas, eps))
-        groups = [dict(params=[p for p in params if is_matrix(p)], matrices=True), dict(params=[p for p in params if not is_matrix(p)], matrices=False)]
-        super().__init__([g for g in groups if g["params"]],
-                         dict(lr=lr, weight_decay=weight_decay, momentum=momentum, betas=betas, eps=eps, steps=steps, matrices=True))
+            if group.get("matrices") and p.dim() < 2:
+                raise ValueError("Muon: a parameter of shape %s is no matrix" % (tuple(p.shape),))
+        known = {id(p) for g in self.param_groups for p in g["params"]}
+        if any(id(tensor(p)) in known for p in params):                      # before the first half of the group is in
+            raise ValueError("Muon: a parameter is in another group already")
+        side = lambda p: group["matrices"] if group.get("matrices") is not None else is_matrix(tensor(p))       # noqa: E731
+        for matrices in (True, False):
+            part = [p for p in params if bool(side(p)) == matrices]
+            if part:
+                super().add_param_group({**group, "params": part, "matrices": matrices})
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -177,3 +177,48 @@ def test_search_step_with_muon(hip):
     *_, losses = st.search_step(0, max_iters=1)
     assert all(torch.isfinite(l).all() for l in losses) and all(torch.isfinite(p).all() for p in st.model.parameters())
     assert sum(not torch.equal(a, b) for a, b in zip(before, st.model.parameters())) > len(before) // 2
+
+
+def test_groups_given_and_added_are_split_and_checked(hip):
+    """A group added later, and groups given as dicts, are split and checked like the parameters of the constructor."""
+    from aadg_amd.muon import Muon, is_matrix
+    net, late = small_net(), nn.Sequential(nn.Conv2d(2, 32, 3, bias=True), nn.Conv2d(32, 32, 3, groups=32), nn.Linear(32, 40)).cuda()
+    a, b = copy.deepcopy(net), copy.deepcopy(late)
+    one = Muon([p for m in (a, b) for p in m.parameters()], lr=0.01)
+    two = Muon(net.parameters(), lr=0.01)
+    two.add_param_group(dict(params=late.parameters(), lr=0.02))
+    three = Muon([dict(params=list(copy.deepcopy(net).parameters()), weight_decay=0.1), dict(params=copy.deepcopy(late)[2].weight, lr=0.02)], lr=0.01)
+    for opt in (one, two, three):
+        for g in opt.param_groups:
+            assert all(is_matrix(p) == g["matrices"] for p in g["params"])
+    assert [(g["lr"], g["matrices"], len(g["params"])) for g in two.param_groups] == [(0.01, True, 2), (0.01, False, 6), (0.02, True, 2), (0.02, False, 4)]
+    assert [(g["lr"], g["weight_decay"], g["matrices"]) for g in three.param_groups] == [(0.01, 0.1, True), (0.01, 0.1, False), (0.02, 0.0, True)]
+    for g in two.param_groups[2:]:
+        g["lr"] = 0.01
+    for m, n in ((a, net), (b, late)):
+        for p, q in zip(m.parameters(), n.parameters()):
+            p.grad = torch.randn_like(p)
+            q.grad = p.grad.clone()
+    one.step()
+    two.step()
+    for m, n in ((a, net), (b, late)):
+        assert all(torch.equal(p, q) for p, q in zip(m.parameters(), n.parameters()))
+    # the group's own word: everything to Adam
+    table = nn.Parameter(torch.zeros(64, 32, device="cuda"))
+    two.add_param_group(dict(params=[table], matrices=False))
+    assert two.param_groups[-1]["matrices"] is False
+    bias = lambda **kw: nn.Parameter(torch.zeros(32, **kw))                                      # noqa: E731
+    with pytest.raises(ValueError):
+        two.add_param_group(dict(params=[bias(device="cuda")], matrices=True))
+    with pytest.raises(ValueError):
+        two.add_param_group(dict(params=[bias(device="cuda")], lr=-1.0))
+    with pytest.raises(ValueError):
+        two.add_param_group(dict(params=[bias(device="cuda")], steps=0))
+    with pytest.raises(ValueError):
+        two.add_param_group(dict(params=[table]))                                           # twice
+    for p in (bias(), bias(device="cuda", dtype=torch.bfloat16)):
+        with pytest.raises(hip.AadgError):
+            two.add_param_group(dict(params=[p]))
+    with pytest.raises(ValueError):
+        Muon([table.detach()])                                                              # nothing to train
+    assert len(two.param_groups) == 5
