@@ -12,10 +12,16 @@ import torch
 from . import _lib
 
 
+def _takes(p):
+    """a matrix of a size that `_lib.orthogonalize` takes"""
+    return p.dim() >= 2 and 0 < p.numel() <= 1 << 28 and max(p.shape[0], p.numel() // p.shape[0]) <= 1 << 16
+
+
 def is_matrix(p):
     """Parameters the orthogonalised update is for: two or more axes, a filter over more than one input channel (depthwise filters are
-    vectors per channel) and at least 16 values along the shorter side (classifier rows and the like stay with Adam)."""
-    return p.dim() >= 2 and p.shape[1] > 1 and min(p.shape[0], p[0].numel()) >= 16
+    vectors per channel), at least 16 values along the shorter side (classifier rows and the like stay with Adam), and a size that
+    `_lib.orthogonalize` takes."""
+    return _takes(p) and p.shape[1] > 1 and min(p.shape[0], p.numel() // p.shape[0]) >= 16
 
 
 class Muon(torch.optim.Optimizer):
@@ -46,8 +52,8 @@ class Muon(torch.optim.Optimizer):
                 raise _lib.AadgError("Muon: parameters must be on one GPU (got %s, %s); there is no CPU path" % (p.device, device))
             if p.dtype != torch.float32:
                 raise _lib.AadgError("Muon: float32 parameters only, got %s" % p.dtype)
-            if group.get("matrices") and p.dim() < 2:
-                raise ValueError("Muon: a parameter of shape %s is no matrix" % (tuple(p.shape),))
+            if group.get("matrices") and not _takes(p):
+                raise ValueError("Muon: a parameter of shape %s has no orthogonalised update" % (tuple(p.shape),))
         known = {id(p) for g in self.param_groups for p in g["params"]}
         if any(id(tensor(p)) in known for p in params):                      # before the first half of the group is in
             raise ValueError("Muon: a parameter is in another group already")
@@ -76,7 +82,9 @@ class Muon(torch.optim.Optimizer):
         bufs, mu, lr = [self.state[p]["momentum"] for p in params], group["momentum"], group["lr"]
         torch._foreach_lerp_(bufs, grads, 1.0 - mu)
         updates = torch._foreach_lerp(grads, bufs, mu)
-        flat = _lib.orthogonalize([u.reshape(u.shape[0], -1) for u in updates], steps=group["steps"])
+        flat = []
+        for i in range(0, len(updates), 4096):                               # (matrices per call of the library)
+            flat += _lib.orthogonalize([u.reshape(u.shape[0], -1) for u in updates[i:i + 4096]], steps=group["steps"])
         out = [o.view(p.shape) for o, p in zip(flat, params)]
         torch._foreach_mul_(out, [-0.2 * lr * max(o.shape) ** 0.5 for o in flat])
         if group["weight_decay"] != 0.0:

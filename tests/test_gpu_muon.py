@@ -222,3 +222,25 @@ def test_groups_given_and_added_are_split_and_checked(hip):
     with pytest.raises(ValueError):
         Muon([table.detach()])                                                              # nothing to train
     assert len(two.param_groups) == 5
+
+
+def test_matrices_past_one_call_of_the_library(hip):
+    """More matrices than one call takes; a matrix longer than the library takes has Adam's update."""
+    from aadg_amd.muon import Muon, is_matrix
+    torch.manual_seed(12)
+    many = [nn.Parameter(torch.randn(16, 17, device="cuda")) for _ in range(4100)]
+    table = nn.Parameter(torch.randn((1 << 16) + 1, 16, device="cuda"))
+    assert is_matrix(many[0]) and not is_matrix(table)
+    opt = Muon(many + [table], lr=0.01)
+    before = [p.detach().clone() for p in many]
+    for p in many + [table]:
+        p.grad = torch.randn_like(p)
+    start = table.detach().clone()
+    opt.step()
+    for i in (0, 4095, 4096, 4099):                                         # U = 0.0975 G
+        want = -0.01 * 0.2 * 17 ** 0.5 * orthogonal64(0.0975 * many[i].grad.double())
+        assert ((many[i] - before[i]).double() - want).abs().max() <= 1e-4 * want.abs().max() + 2.0 ** -23 * before[i].abs().max()
+    # Adam's first step: lr g / (|g| + eps) up to rounding
+    assert ((table - start) + 0.01 * table.grad.sign()).abs().max() <= 2.0 ** -23 * start.abs().max() + 0.01 * 1e-8 / table.grad.abs().min()
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[nn.Parameter(torch.zeros((1 << 16) + 1, 16, device="cuda"))], matrices=True))

@@ -26,3 +26,10 @@ def test_which_parameters_are_matrices():
     yes = [(64, 64), (16, 16), (64, 3, 7, 7), (64, 16, 1, 1)]
     no = [(64,), (), (2, 768), (64, 1, 3, 3), (15, 400), (64, 8), (2, 256, 1, 1)]
     assert all(is_matrix(torch.zeros(s)) for s in yes) and not any(is_matrix(torch.zeros(s)) for s in no)
+
+
+def test_sizes_outside_the_library_stay_with_adam():
+    from aadg_amd.muon import is_matrix
+    no = [(0, 64), (64, 0), ((1 << 16) + 1, 16), (16, (1 << 16) + 1), (1 << 15, (1 << 13) + 1)]
+    assert not any(is_matrix(torch.empty(s, device="meta")) for s in no)
+    assert all(is_matrix(torch.empty(s, device="meta")) for s in [(1 << 16, 16), (16, 1 << 16), (1 << 15, 1 << 13)])
