@@ -65,6 +65,8 @@ class Muon(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.AadgError("Muon: step() cannot be captured into a graph (learning rate and step count are host values)")
         loss = None
         if closure is not None:
             with torch.enable_grad():

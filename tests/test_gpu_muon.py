@@ -244,3 +244,20 @@ def test_matrices_past_one_call_of_the_library(hip):
     assert ((table - start) + 0.01 * table.grad.sign()).abs().max() <= 2.0 ** -23 * start.abs().max() + 0.01 * 1e-8 / table.grad.abs().min()
     with pytest.raises(ValueError):
         opt.add_param_group(dict(params=[nn.Parameter(torch.zeros((1 << 16) + 1, 16, device="cuda"))], matrices=True))
+
+
+def test_a_captured_step_is_refused(hip, monkeypatch):
+    """the learning rate and Adam's step count are host values: a captured step would repeat them on every replay"""
+    from aadg_amd.muon import Muon
+    net = small_net()
+    opt = Muon(net.parameters(), lr=0.01)
+    for p in net.parameters():
+        p.grad = torch.randn_like(p)
+    before = [p.detach().clone() for p in net.parameters()]
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(hip.AadgError):
+            opt.step()
+    assert all(torch.equal(a, b) for a, b in zip(before, net.parameters())) and not opt.state
+    opt.step()
+    assert not any(torch.equal(a, b) for a, b in zip(before, net.parameters()))
