@@ -117,7 +117,8 @@ def attention(q, k, v, scale=None, causal=False, key_lengths=None):
 
     key_lengths: int32 [B] on the device, clamped to 0 ... Nk: keys and values behind a sequence's length are not used, whatever they hold.
     causal: query i of a sequence with L keys sees keys j <= i + L - Nq (the last query sees every key).  A query that sees no key
-    gives zeros and takes no part in any gradient.  Inputs are expected finite (a key that only the causal rule hides included).
+    gives zeros and takes no part in any gradient, whatever it and its output's gradient hold.  Other inputs are expected finite (a key that
+    only the causal rule hides included).
 
     Returns [B, H, Nq, d] over [B, Nq, H, d] memory: `.transpose(1, 2).reshape(B, Nq, H * d)` is free.  Differentiable once in q, k, v, in reverse mode (a
     forward-mode tangent raises NotImplementedError)."""

@@ -189,12 +189,16 @@ __device__ __forceinline__ int at_limit_max(const AtArgs& a, int L, int row0, in
 // waves per SIMD the registers are budgeted for: two (256 registers), one for head widths over 64
 template <typename T, int D> constexpr int at_min_waves() { return D == 128 ? 1 : 2; }
 
-// keys per LDS tile: 64; 32 where the next tile's prefetch registers (2 BK D / threads values) would not fit beside the accumulators
+// keys per LDS tile: 64; 32 where the next tile's prefetch registers (2 BK D / threads values) would not fit beside the accumulators.  The one-wave float32
+// backward (up to 32 rows or keys) is over its 256 registers all the same: k_attn_dkv<float, 64, 1> keeps 31 of them in memory, k_attn_dq<float, 64, 1>
+// 16 ... 18, k_attn_dkv_pair<float, 128, 2> 6.
 template <typename T, int D, int NW> constexpr int at_bk() { return NW == 1 || (sizeof(T) == 4 && D == 128) ? 32 : 64; }
 
 // group and row tile of a workgroup.  Causal: by the length of the tiles' rows, all groups and heads side by side, the longest first, so that the
-// launch does not end in long tiles; where every workgroup has a place at once (two a CU, number i and i + 256) the second half backwards,
-// so that a CU has a long and a short one.  (Tiles of a head: the r heads' in turn, exact where Nq is a multiple of the tile.)
+// launch does not end in long tiles; up to 512 workgroups, which all have a place at once where a CU takes two (number i and i + 256), the second half
+// backwards, so that a CU has a long and a short one.  Two waves a SIMD is what bfloat16 width 128 and float32 width 64 run, the kernels that gain
+// (two causal sequences of 4096, D = 128, forward and backward: 655 -> 600 us); bfloat16 widths of 64 and 32 have three and four (768 and 1024 places),
+// float32 width 128 one, where the order is only another one.  (Tiles of a head: the r heads' in turn, exact where Nq is a multiple of the tile.)
 __device__ __forceinline__ void at_row_tile(const AtArgs& a, int w, bool split, int& bg, int& tile) {
     if (!a.causal || split) {
         bg = w / a.tiles;
@@ -213,10 +217,11 @@ __device__ __forceinline__ void at_row_tile(const AtArgs& a, int w, bool split, 
 
 // ------------------------------------------------------------------------------------------------ forward
 // Workgroup: NW waves of 32 folded rows; keys in tiles of BK through LDS, the next tile's loads in registers during the products.
-// Bound by the vector units in bfloat16: a score costs as many of their cycles (exponential, maximum, sum, packing) as D / 32 matrix
-// instructions' share.  48 x 16384 rows, 256 keys, D = 64: 98 us, 0.53 PFLOP/s (vector issue 0.66 of the time, matrix 0.26); two causal sequences of
-// 8192, 16 heads over 4, D = 128: 607 us, 0.91 PFLOP/s (800 us with each head's tiles in a row).  In float32 by the matrix units: 240 x 1024 rows, 256 keys, D = 64: 157 us,
-// 103 TFLOP/s of the 153 that a large float32 product reaches.  A workgroup that holds all 256
+// Times in a loop of calls (single launches of the larger shapes take a tenth more under a profiler).  bfloat16, 48 x 16384 rows, 256 keys, D = 64: 98 us,
+// 0.53 PFLOP/s: vector instructions issue in 0.66 of a CU's busy cycles (exponential, maximum, sum, packing: as many a score as D / 32 matrix
+// instructions' share), the matrix units work in 0.26, waves wait 0.30 of their time -- no unit is at its limit.  Two causal sequences of 8192, 16 heads over
+// 4, D = 128: 580 ... 607 us on two boxes, 0.91 ... 0.95 PFLOP/s, vector 0.57, matrix 0.47 (800 us with each head's tiles in a row).  float32, 240 x 1024 rows, 256
+// keys, D = 64: 155 us, 104 TFLOP/s of the 153 that a large float32 product reaches, matrix units 0.74.  A workgroup that holds all 256
 // keys takes 88 us for the first case, but there is one to a CU and rows are cut into whole rounds of them (96 groups: 3/4 of the CUs), so this form
 // serves every shape.  Two row blocks a wave take the same time.
 template <typename T, int D, int NW, bool SPLIT>
@@ -744,7 +749,8 @@ __global__ __launch_bounds__(64 * NW, (at_min_waves<T, D>())) void k_attn_dkv(co
 // S = Q K^T, makes P and hands it over through LDS (lane to lane, float32), then accumulates dv^T += dO^T P; wave 1 keeps V, takes dP = dO V^T - D
 // (-D_i is the initial value of its accumulators), makes dS = P dP and accumulates dk^T += Q^T dS.  Both halves are the same code on swapped
 // operands and the same number of products; one wave doing both needs 2 D accumulator and D fragment registers and leaves a SIMD one
-// wave (two causal sequences of 4096, 8 heads over 2, D = 128: 264 us, 0.52 PFLOP/s; in pieces half as fine 365 us, 423 in one wave).
+// wave (two causal sequences of 4096, 8 heads over 2, D = 128: 263 us, 0.52 PFLOP/s, vector 0.39, matrix 0.26 of the time; in pieces half as fine 365 us, 423 in
+// one wave).
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
     typedef At<T> M;
@@ -912,7 +918,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_dkv_pair(const AtArgs a) {
 // ([key][row], 72 bytes a key: 8-byte writes of neighbouring keys and the transpose reads spread over the banks), and dq^T = K^T dS^T is taken in
 // 16 x 16 tiles (v_mfma_f32_16x16x32_bf16: every wave has its tiles over all keys, no sum across waves; its K^T fragments stay in registers).
 // D_i comes from the rows on their way to LDS (eight neighbouring lanes hold a row).
-// 48 x 16384 rows, 256 keys, D = 64: 206 us, 0.63 PFLOP/s (139 + 172 us in two walks); vector issue 0.42, LDS 0.40, matrix 0.33 of the time: two
+// 48 x 16384 rows, 256 keys, D = 64: 207 us, 0.62 PFLOP/s (139 + 172 us in two walks); vector issue 0.41, LDS 0.38, matrix 0.32 of the time: two
 // barriers a tile of 32 rows, which software pipelining over one barrier did not shorten.
 template <int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, 2) void k_attn_bwd_short(const AtArgs a) {

@@ -11,8 +11,9 @@
 // more, summed in float32 on the bfloat16 matrix cores -- six at 16 times the rate of the float32 matrix instructions.  The planes are
 // written by the kernel that produces a matrix, once per element; the product kernels move bfloat16 only.
 //
-// All matrices of the list go through each phase in ONE launch: a workgroup finds its matrix from the running tile counts of a table in the
-// workspace.  The table travels in kernel arguments (26 entries a launch), so a captured graph keeps it.
+// All matrices of a group (or_group: two) go through each phase in ONE launch: a workgroup finds its matrix from the running tile counts of a table in the
+// workspace.  The table travels in kernel arguments, one launch for 26 entries, so a captured graph keeps it.  Five steps of one matrix or of 26 of
+// a group: 18 launches (near square), 20 (wide, 22 where long products are cut).
 #include <algorithm>
 
 #include "common.h"

@@ -639,7 +639,8 @@ int aadg_upsample_sum_backward_all(const void* dout, void* const* dlows, const i
  * stride a multiple of 16 bytes; 0 < scale < inf.  Keys and values behind L_b are never used.  lse [B, H, Nq] float32: log2 of the
  * softmax denominators (+inf for a row without keys), written by the forward (NULL: not), read by the backward.
  * Backward: from dout [B, H, Nq, d] dq, dk, dv (dq NULL, or dk and dv NULL: not computed); dk / dv are summed over the heads that
- * share a key head and are zero behind L_b.  Sums have a fixed order: equal inputs give equal bits.
+ * share a key head and are zero behind L_b; rows that see no key reach no gradient, whatever q and dout hold there.  Sums have a fixed
+ * order: equal inputs give equal bits.
  * ------------------------------------------------------------------------------------------- */
 typedef struct aadg_attention_desc {
     int32_t dtype, B, H, G, Nq, Nk, d, causal;
