@@ -261,3 +261,17 @@ def test_a_captured_step_is_refused(hip, monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(before, net.parameters())) and not opt.state
     opt.step()
     assert not any(torch.equal(a, b) for a, b in zip(before, net.parameters()))
+
+
+def test_named_parameters(hip):
+    from aadg_amd.muon import Muon, is_matrix
+    net = small_net()
+    twin = copy.deepcopy(net)
+    opt, plain = Muon(net.named_parameters(), lr=0.01), Muon(twin.parameters(), lr=0.01)
+    assert sum((g["param_names"] for g in opt.param_groups), []) == sorted(dict(net.named_parameters()), key=lambda n: not is_matrix(net.get_parameter(n)))
+    for p, q in zip(net.parameters(), twin.parameters()):
+        p.grad = torch.randn_like(p)
+        q.grad = p.grad.clone()
+    opt.step()
+    plain.step()
+    assert all(torch.equal(p, q) for p, q in zip(net.parameters(), twin.parameters()))
