@@ -41,8 +41,8 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("Muon: lr %r, weight_decay %r, momentum %r, betas %r, eps %r, steps %r" % (lr, wd, momentum, betas, eps, steps))
         params = [group["params"]] if torch.is_tensor(group["params"]) else list(group["params"])
         tensor = lambda p: p[1] if isinstance(p, tuple) else p                                  # noqa: E731  (name, parameter)
-        if not all(torch.is_tensor(tensor(p)) for p in params):
-            raise TypeError("Muon: parameters must be tensors")
+        if isinstance(group["params"], set) or not all(torch.is_tensor(tensor(p)) for p in params):
+            raise TypeError("Muon: parameters must be tensors, in an order")
         params = [p for p in params if tensor(p).requires_grad]
         if not params:
             raise ValueError("Muon: no parameter of the group requires a gradient")
@@ -54,9 +54,9 @@ class Muon(torch.optim.Optimizer):
                 raise _lib.AadgError("Muon: float32 parameters only, got %s" % p.dtype)
             if group.get("matrices") and not _takes(p):
                 raise ValueError("Muon: a parameter of shape %s has no orthogonalised update" % (tuple(p.shape),))
-        known = {id(p) for g in self.param_groups for p in g["params"]}
-        if any(id(tensor(p)) in known for p in params):                      # before the first half of the group is in
-            raise ValueError("Muon: a parameter is in another group already")
+        known = {id(p) for g in self.param_groups for p in g["params"]}      # (what torch refuses, before half of the group is in)
+        if any(id(p) in known or not (p.is_leaf or p.retains_grad) for p in map(tensor, params)):
+            raise ValueError("Muon: a parameter is in another group already, or no leaf")
         side = lambda p: group["matrices"] if group.get("matrices") is not None else is_matrix(tensor(p))       # noqa: E731
         for matrices in (True, False):
             part = [p for p in params if bool(side(p)) == matrices]

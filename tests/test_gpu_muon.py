@@ -275,3 +275,13 @@ def test_named_parameters(hip):
     opt.step()
     plain.step()
     assert all(torch.equal(p, q) for p, q in zip(net.parameters(), twin.parameters()))
+
+
+def test_a_refused_group_leaves_the_optimizer_as_it_was(hip):
+    from aadg_amd.muon import Muon
+    w = lambda: nn.Parameter(torch.zeros(32, 32, device="cuda"))                                 # noqa: E731
+    opt = Muon([w()])
+    for params, error in (([w(), torch.zeros(32, device="cuda", requires_grad=True) * 2], ValueError), ({w(), w()}, TypeError), ([w(), "bias"], TypeError)):
+        with pytest.raises(error):
+            opt.add_param_group(dict(params=params))
+        assert len(opt.param_groups) == 1
