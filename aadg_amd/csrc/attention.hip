@@ -220,7 +220,7 @@ __device__ __forceinline__ void at_row_tile(const AtArgs& a, int w, bool split, 
 // Times in a loop of calls (single launches of the larger shapes take a tenth more under a profiler).  bfloat16, 48 x 16384 rows, 256 keys, D = 64: 98 us,
 // 0.53 PFLOP/s: vector instructions issue in 0.66 of a CU's busy cycles (exponential, maximum, sum, packing: as many a score as D / 32 matrix
 // instructions' share), the matrix units work in 0.26, waves wait 0.30 of their time -- no unit is at its limit.  Two causal sequences of 8192, 16 heads over
-// 4, D = 128: 580 ... 607 us on two boxes, 0.91 ... 0.95 PFLOP/s, vector 0.57, matrix 0.47 (800 us with each head's tiles in a row).  float32, 240 x 1024 rows, 256
+// 4, D = 128: 580 ... 607 us on two cards, 0.91 ... 0.95 PFLOP/s, vector 0.57, matrix 0.47 (800 us with each head's tiles in a row).  float32, 240 x 1024 rows, 256
 // keys, D = 64: 155 us, 104 TFLOP/s of the 153 that a large float32 product reaches, matrix units 0.74.  A workgroup that holds all 256
 // keys takes 88 us for the first case, but there is one to a CU and rows are cut into whole rounds of them (96 groups: 3/4 of the CUs), so this form
 // serves every shape.  Two row blocks a wave take the same time.
